@@ -203,10 +203,10 @@ def _own_adamw(s):
     c = s["case"]
     opt = s.get("optimizer")
     if opt is None:                              # a program builds its optimizer once
-        opt = s["optimizer"] = AdamW(s["params"], lr=LR, betas=(B1, B2), eps=EPS, weight_decay=DECAY, state_bits=c["bits"], copies=s["copies"], seed=SEED)
+        opt = s["optimizer"] = AdamW(s["params"], s["grads"], lr=LR, betas=(B1, B2), eps=EPS, weight_decay=DECAY, state_bits=c["bits"], copies=s["copies"], seed=SEED)
         held = {"m": s["qm"], "v": s["qv"], "m_scale": s["m_scale"], "v_scale": s["v_scale"]} if c["bits"] == 8 else {"m": s["m"], "v": s["v"]}
         opt.set_state(t=s["t"], **held)
-    opt.step(s["grads"], grad_scale=1.0 / GRAD_SCALE[c["grad"]])
+    opt.step(grad_scale=1.0 / GRAD_SCALE[c["grad"]])
     if c["bits"] == 8:                           # the states as the values that they stand for
         opt.moments(out=(s["m"], s["v"]))
     return {k: s["arena"][k] for k in ("params", "m", "v", "copies") if k in s["arena"]}
