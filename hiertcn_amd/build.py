@@ -13,7 +13,8 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libhiertcn_gfx950.so")
 SOURCES = ["api.hip", "prep.hip", "pool_gru.hip", "gru_persist.hip", "tcn.hip", "tcn_layers.hip", "score.hip", "score_bwd.hip", "metrics.hip", "train.hip", "gmm.hip", "gmm_train.hip", "gmm_gram.hip", "exact.hip", "gemm.hip", "gru_x3.hip", "score_x3.hip", "score_x3w.hip", "lgru_tile.hip", "lgru_pipe.hip", "lgru_wide.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-Wno-pass-failed", "-Wno-shift-negative-value",
-         "-fno-gpu-rdc", "-D__HIP_PLATFORM_AMD__"]
+         "-fno-gpu-rdc", "-D__HIP_PLATFORM_AMD__",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]   # no packed fp32 arithmetic: some of its forms have given wrong results on this hardware now and then
 
 
 def _hipcc():

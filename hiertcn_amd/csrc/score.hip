@@ -458,7 +458,7 @@ struct RowState2 {
   float s;     // sum of 2^(z*log2(e) - m2)
   int c;       // count of z > t
   float xp, ep, ssave;  // PMODE 5: software-pipeline registers (pending exponent, pending term) and the tile checkpoint of s
-  f32x2 s2, xp2, ep2;   // PMODE 7/8: the same pipeline on PAIRS of logits (v_pk_fma_f32 / v_pk_add_f32: two values per issue slot)
+  f32x2 s2, xp2, ep2;   // PMODE 7/8: the same pipeline on PAIRS of logits
   unsigned bits;        // PMODE 7: sign bits of (t - z) of the current tile, one per logit (popcount at the end of the tile)
 };
 
@@ -467,9 +467,9 @@ struct RowState2 {
 // 5 full, epilogue software-pipelined across values (the fma / exp / add of one logit sit in three consecutive
 // MFMA gaps, so no VALU op waits on the one before it) and the reference moved only when the running sum
 // overflows (checked once per tile; the tile is then redone from its checkpoint with a new reference).
-// 7: as 5 on pairs of logits with the packed fp32 ops (fma and sum cost half an issue slot per logit) and the count taken
-// from the sign of (t - z) shifted into a bit register (v_pk_add + v_alignbit, popcount once per tile) instead of
-// v_cmp + v_addc; 8: packed sum, compare/add-carry count.
+// 7: as 5 on pairs of logits and the count taken
+// from the sign of (t - z) shifted into a bit register (a subtraction + v_alignbit, popcount once per tile) instead of
+// v_cmp + v_addc; 8: as 7 with a compare/add-carry count.
 // NB = 32-step blocks per wave, NSTG = LDS stages: <2, 3> for C <= 256; <1, 2> for C = 512, where 64 rows of resident B operand
 // would take all 256 VGPRs and three 64 KB stages do not fit the 160 KB of LDS.
 // PAD (C >= 256): the LDS image of a stage is padded per 1 KB LDS-DMA piece instead of XOR-swizzled per row, so that the A fragment of
@@ -580,7 +580,7 @@ __global__ __launch_bounds__(SC_THREADS, 2) void k_score_pipe(const uint16_t* __
     st[cbk].xp = st[cbk].ep = st[cbk].ssave = 0.f;
     st[cbk].s2 = st[cbk].xp2 = st[cbk].ep2 = f32x2{0.f, 0.f};
     st[cbk].bits = 0u;
-    if (PMODE == 7 || PMODE == 9) st[cbk].t = t + 0.0f;   // -0 -> +0: then (t - z) is negative exactly when z > t (no -0 result possible)
+    if (PMODE == 7) st[cbk].t = t + 0.0f;   // -0 -> +0: then (t - z) is negative exactly when z > t (no -0 result possible)
   }
 
   const int n_all = NP / SC_STAGE;
@@ -699,29 +699,9 @@ __global__ __launch_bounds__(SC_THREADS, 2) void k_score_pipe(const uint16_t* __
   };
   // PMODE 7/8: gap i of a tile handles pair j = i/2.  Even gap: s2 += e2(j-2); e(j-1).lo = 2^x(j-1).lo; d2 = t - v2(j).
   // Odd gap: e(j-1).hi = 2^x(j-1).hi; x2(j) = v2(j)*log2(e) - m2.  Every gap: one sign bit into rs.bits.
-  // PMODE 9 = 7 with the packed ops written in asm: hipcc (SIPreEmitPeephole) splits v_pk_*_f32 that sit behind an MFMA back
-  // into two scalar ops on gfx950, so 7 as compiled is only partly packed.
-  auto pk_add = [&](f32x2 a, f32x2 b) { f32x2 r; asm volatile("v_pk_add_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; };
   auto val7 = [&](int i, const f32x16& v, RowState2& rs, f32x2& d2) {
     const int j = i >> 1;
     const f32x2 v2 = {v[2 * j], v[2 * j + 1]};
-    if (PMODE == 9) {
-      const f32x2 tm = {rs.t, rs.m2};
-      const f32x2 l2 = {LOG2E_F, LOG2E_F};
-      if ((i & 1) == 0) {
-        if (j >= 2) rs.s2 = pk_add(rs.s2, rs.ep2);
-        if (j >= 1) rs.ep2.x = __builtin_amdgcn_exp2f(rs.xp2.x);
-        asm volatile("v_pk_add_f32 %0, %1, %2 op_sel_hi:[0,1] neg_lo:[0,1] neg_hi:[0,1]" : "=v"(d2) : "v"(tm), "v"(v2));
-        rs.bits = (i == 0) ? (__float_as_uint(d2.x) >> 31) : __builtin_amdgcn_alignbit(rs.bits, __float_as_uint(d2.x), 31);
-      } else {
-        if (j >= 1) rs.ep2.y = __builtin_amdgcn_exp2f(rs.xp2.y);
-        asm volatile("v_pk_fma_f32 %0, %1, %2, %3 op_sel:[0,0,1] op_sel_hi:[1,0,1] neg_lo:[0,0,1] neg_hi:[0,0,1]"
-                     : "=v"(rs.xp2) : "v"(v2), "s"(l2), "v"(tm));
-        rs.bits = __builtin_amdgcn_alignbit(rs.bits, __float_as_uint(d2.y), 31);
-      }
-      asm volatile("" : "+v"(rs.s2), "+v"(rs.c), "+v"(rs.ep2), "+v"(rs.xp2), "+v"(rs.bits), "+v"(d2));
-      return;
-    }
     if ((i & 1) == 0) {
       if (j >= 2) rs.s2 += rs.ep2;
       if (j >= 1) rs.ep2.x = __builtin_amdgcn_exp2f(rs.xp2.x);
@@ -744,7 +724,7 @@ __global__ __launch_bounds__(SC_THREADS, 2) void k_score_pipe(const uint16_t* __
     rs.ep2.x = __builtin_amdgcn_exp2f(rs.xp2.x);
     rs.ep2.y = __builtin_amdgcn_exp2f(rs.xp2.y);
     rs.s2 += rs.ep2;
-    if (PMODE == 7 || PMODE == 9) rs.c += __builtin_popcount(rs.bits);
+    if (PMODE == 7) rs.c += __builtin_popcount(rs.bits);
     const float tot = rs.s2.x + rs.s2.y;
     if (__any(!(tot < 1.0e38f))) {
       float tm = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
@@ -1502,7 +1482,6 @@ static hipError_t launch_score_c(const ModelDev& m, const uint16_t* hidden, cons
   if (pvar && pvar[0] == '6') return launch_score_pipe<C, 6>(m, hidden, y, R, out, st);
   if (pvar && pvar[0] == '7') return launch_score_pipe<C, 7>(m, hidden, y, R, out, st, row_map, n_rows_dev, split_scratch);
   if (pvar && pvar[0] == '8') return launch_score_pipe<C, 8>(m, hidden, y, R, out, st, row_map, n_rows_dev, split_scratch);
-  if (pvar && pvar[0] == '9') return launch_score_pipe<C, 9>(m, hidden, y, R, out, st, row_map, n_rows_dev, split_scratch);
   if (C == 256 && pvar && pvar[0] == 'c') return launch_score_pipe<256, 12, 2, 3, true>(m, hidden, y, R, out, st, row_map, n_rows_dev, split_scratch);
   if (C == 256 && pvar && pvar[0] == 'd') return launch_score_pipe<256, 13, 2, 3, true>(m, hidden, y, R, out, st, row_map, n_rows_dev, split_scratch);
   if (C == 256 && pvar && pvar[0] == 'h') return launch_score_pipe<256, 16, 2, 3, true>(m, hidden, y, R, out, st, row_map, n_rows_dev, split_scratch);
