@@ -1,0 +1,156 @@
+"""AdamW (Adam with decoupled weight decay) over many tensors in one or a few launches, moments in 32 or in 8 bits.  Beside the handles' own TF-form Adam
+(Engine.adam_step, model.py:139), which has neither.  Kernel: csrc/adamw.hip; exact formulas: include/hiertcn_ops.h."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import List, Optional, Sequence, Union
+
+import torch
+
+from . import _ops
+from ._lib import HierTCNError
+from ._ops import need
+
+BLOCK = 256      # elements that share a scale of the 8-bit states
+
+
+class AdamW:
+    """params: fp32 masters (contiguous, on one GPU).  grads: where every step finds the gradients (fp32 / bf16 / fp16, None: no gradient) -- or give them to
+    step().  copies: 16-bit tensors that receive the rounded parameters in the same pass (None entries: none).  weight_decay: one value, or one per
+    tensor.  state_bits 32: m, v fp32 (8 bytes a parameter); 8: codes with a scale per 256 elements (2 bytes a parameter), rounded at random such that
+    the expected state is exact -- `seed` and the step number determine the random bits, so runs repeat.
+
+    The step number is the object's (`t`), so a step cannot be captured into a graph (it would replay with the same bias corrections): it is refused
+    there, as the framework's graphs leave Adam outside."""
+
+    def __init__(self, params: Sequence[torch.Tensor], grads: Optional[Sequence[Optional[torch.Tensor]]] = None, lr: float = 1e-3, betas=(0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: Union[float, Sequence[float]] = 0.0, state_bits: int = 32,
+                 copies: Optional[Sequence[Optional[torch.Tensor]]] = None, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise HierTCNError(f"state_bits {state_bits}: 8 or 32")
+        self.params: List[torch.Tensor] = list(params)
+        if not self.params:
+            raise HierTCNError("no parameters")
+        n = len(self.params)
+        self.device = _ops.on_gpu(self.params[0], "params[0]")
+        for i, p in enumerate(self.params):
+            need(p, f"params[{i}]", torch.float32, self.device, p.shape if isinstance(p, torch.Tensor) else ())
+        decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+        copies = [None] * n if copies is None else list(copies)
+        if len(decay) != n or len(copies) != n:
+            raise HierTCNError(f"{n} parameters, {len(decay)} weight decays, {len(copies)} copies")
+        self.lr, self.betas, self.eps, self.state_bits, self.seed, self.t = float(lr), (float(betas[0]), float(betas[1])), float(eps), state_bits, int(seed), 0
+        self.weight_decay, self.copies = decay, copies
+        self._desc = (_ops.AdamwTensor * n)()
+        for i, (p, c, d) in enumerate(zip(self.params, copies, self._desc)):
+            d.numel, d.param, d.weight_decay, d.index = p.numel(), p.data_ptr(), decay[i], i
+            if c is not None:
+                if not isinstance(c, torch.Tensor) or c.dtype not in (torch.bfloat16, torch.float16):
+                    raise HierTCNError(f"copies[{i}]: a bfloat16 or float16 tensor")
+                d.copy, d.copy_dtype = need(c, f"copies[{i}]", c.dtype, self.device, p.shape).data_ptr(), _ops.DTYPE[c.dtype]
+        zeros = lambda dt, block=1: [torch.zeros(-(-p.numel() // block), dtype=dt, device=self.device) for p in self.params]  # noqa: E731
+        if state_bits == 32:
+            self._attach(zeros(torch.float32), zeros(torch.float32), None, None)
+        else:
+            self._attach(zeros(torch.int8), zeros(torch.uint8), zeros(torch.float32, BLOCK), zeros(torch.float32, BLOCK))
+        self.grads = None
+        if grads is not None:
+            self._bind(grads)
+            self.grads = list(grads)
+
+    def _attach(self, m, v, m_scale, v_scale):
+        dm, dv = (torch.float32, torch.float32) if self.state_bits == 32 else (torch.int8, torch.uint8)
+        for i, (p, d) in enumerate(zip(self.params, self._desc)):
+            k, blocks = torch.Size([p.numel()]), torch.Size([-(-p.numel() // BLOCK)])
+            d.m, d.v = need(m[i], f"m[{i}]", dm, self.device, k).data_ptr(), need(v[i], f"v[{i}]", dv, self.device, k).data_ptr()
+            if self.state_bits == 8:
+                d.m_scale = need(m_scale[i], f"m_scale[{i}]", torch.float32, self.device, blocks).data_ptr()
+                d.v_scale = need(v_scale[i], f"v_scale[{i}]", torch.float32, self.device, blocks).data_ptr()
+        self.m, self.v, self.m_scale, self.v_scale = m, v, m_scale, v_scale
+
+    def set_state(self, m, v, t: int, m_scale=None, v_scale=None):
+        """Takes flat tensors as the states THEMSELVES (no copy): fp32 moments, or int8 / uint8 codes with their scales [ceil(numel / 256)]; t: steps taken."""
+        lists = [list(x) if x is not None else None for x in (m, v, m_scale, v_scale)]
+        if any(x is not None and len(x) != len(self.params) for x in lists) or None in lists[:2] or (self.state_bits == 8) != (None not in lists[2:]):
+            raise HierTCNError("one m and one v per parameter, and a scale of each with 8-bit states only")
+        if int(t) < 0:
+            raise HierTCNError(f"t = {t}")
+        self._attach(*lists)
+        self.t = int(t)
+
+    def state_dict(self) -> dict:
+        """t, seed and the states on the host (checkpoints)."""
+        out = dict(t=self.t, seed=self.seed, state_bits=self.state_bits, m=[x.cpu() for x in self.m], v=[x.cpu() for x in self.v])
+        if self.state_bits == 8:
+            out.update(m_scale=[x.cpu() for x in self.m_scale], v_scale=[x.cpu() for x in self.v_scale])
+        return out
+
+    def load_state_dict(self, state: dict):
+        """Copies a state_dict() into the states."""
+        names = ("m", "v") + (("m_scale", "v_scale") if self.state_bits == 8 else ())
+        if int(state["state_bits"]) != self.state_bits or any(len(state[k]) != len(self.params) for k in names):
+            raise HierTCNError("the state belongs to another optimizer (state_bits or number of tensors)")
+        pairs = [(a, b) for k in names for a, b in zip(getattr(self, k), state[k])]
+        if any(a.shape != b.shape or a.dtype != b.dtype for a, b in pairs):
+            raise HierTCNError("the state belongs to other tensors")
+        for a, b in pairs:
+            a.copy_(b)
+        self.t, self.seed = int(state["t"]), int(state["seed"])
+
+    def _bind(self, grads):
+        if len(grads) != len(self.params):
+            raise HierTCNError(f"{len(self.params)} parameters, {len(grads)} gradients")
+        for i, (p, g, d) in enumerate(zip(self.params, grads, self._desc)):
+            if g is None:
+                d.grad = None
+                continue
+            if not isinstance(g, torch.Tensor) or g.dtype not in _ops.DTYPE:
+                raise HierTCNError(f"grads[{i}]: a float32, bfloat16 or float16 tensor")
+            d.grad, d.grad_dtype = need(g, f"grads[{i}]", g.dtype, self.device, p.shape).data_ptr(), _ops.DTYPE[g.dtype]
+
+    def step(self, grads: Optional[Sequence[Optional[torch.Tensor]]] = None, lr: Optional[float] = None, grad_scale: Union[float, torch.Tensor] = 1.0):
+        """One step.  grads: this step's (default: the buffers given to the constructor); a parameter without one is left as it is.  grad_scale multiplies
+        every gradient: a number, or a device float32 tensor of one element (clipping by the global norm)."""
+        if grads is not None:
+            self._bind(grads)
+        elif self.grads is None:
+            raise HierTCNError("no gradients: give them to step() or to the constructor")
+        a = _ops.Adamw(lr=self.lr if lr is None else float(lr), beta1=self.betas[0], beta2=self.betas[1], eps=self.eps, grad_scale=1.0, t=self.t + 1,
+                       seed=self.seed, state_bits=self.state_bits)
+        if isinstance(grad_scale, torch.Tensor):
+            if grad_scale.numel() != 1:
+                raise HierTCNError(f"grad_scale: {grad_scale.numel()} elements, expected one")
+            a.grad_scale_dev = need(grad_scale, "grad_scale", torch.float32, self.device, grad_scale.shape).data_ptr()
+        else:
+            a.grad_scale = float(grad_scale)
+        try:
+            _ops.call(_ops.lib().hiertcn_adamw_step, self.device, self._desc, len(self._desc), C.byref(a))
+        finally:
+            if grads is not None and self.grads is not None:
+                self._bind(self.grads)
+        self.t += 1
+
+    def moments(self, out=None):
+        """-> (m, v): lists of flat fp32 tensors -- the states themselves (32 bits), or the values that the codes stand for, written to `out` = (list, list)
+        where that is given (entries of None are skipped)."""
+        if self.state_bits == 32:
+            if out is not None:
+                for dst, src in zip((*out[0], *out[1]), (*self.m, *self.v)):
+                    if dst is not None:
+                        dst.copy_(src)
+                return out
+            return self.m, self.v
+        n = len(self.params)
+        if out is None:
+            out = tuple([torch.empty(p.numel(), dtype=torch.float32, device=self.device) for p in self.params] for _ in range(2))
+        if len(out[0]) != n or len(out[1]) != n:
+            raise HierTCNError(f"{n} parameters, outputs for {len(out[0])} and {len(out[1])}")
+        ptrs = []
+        for name, lst in zip("mv", out):
+            arr = (C.c_void_p * n)()
+            for i, (o, p) in enumerate(zip(lst, self.params)):
+                if o is not None:
+                    arr[i] = need(o, f"out {name}[{i}]", torch.float32, self.device, torch.Size([p.numel()])).data_ptr()
+            ptrs.append(arr)
+        _ops.call(_ops.lib().hiertcn_adamw_moments, self.device, self._desc, n, *ptrs)
+        return out

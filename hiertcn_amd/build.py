@@ -11,7 +11,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libhiertcn_gfx950.so")
-SOURCES = ["api.hip", "prep.hip", "pool_gru.hip", "gru_persist.hip", "tcn.hip", "tcn_layers.hip", "score.hip", "score_bwd.hip", "metrics.hip", "train.hip", "gmm.hip", "gmm_train.hip", "gmm_gram.hip", "exact.hip", "gemm.hip", "gru_x3.hip", "score_x3.hip", "score_x3w.hip", "lgru_tile.hip", "lgru_pipe.hip", "lgru_wide.hip"]
+SOURCES = ["api.hip", "prep.hip", "pool_gru.hip", "gru_persist.hip", "tcn.hip", "tcn_layers.hip", "score.hip", "score_bwd.hip", "metrics.hip", "train.hip", "gmm.hip", "gmm_train.hip", "gmm_gram.hip", "exact.hip", "gemm.hip", "gru_x3.hip", "score_x3.hip", "score_x3w.hip", "lgru_tile.hip", "lgru_pipe.hip", "lgru_wide.hip",
+           "ops.hip", "glr.hip", "seq_loss.hip", "adamw.hip"]
+OPS_SOURCES = ("ops.hip", "glr.hip", "seq_loss.hip", "adamw.hip")   # the sequence operators (include/hiertcn_ops.h)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-Wno-pass-failed", "-Wno-shift-negative-value",
          "-fno-gpu-rdc", "-D__HIP_PLATFORM_AMD__",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]   # no packed fp32 arithmetic: some of its forms have given wrong results on this hardware now and then
@@ -92,6 +94,10 @@ def _headers():
         os.path.join(HERE, "..", "include", "hiertcn.h")]
 
 
+def _ops_headers(src: str):
+    return [os.path.join(CSRC, "ops.h"), os.path.join(HERE, "..", "include", "hiertcn_ops.h")] if src in OPS_SOURCES or src == "api.hip" else []
+
+
 LIB_PACKER = os.path.join(HERE, "libhiertcn_packer.so")   # host-side batch packer (csrc/packer.c: plain C, gcc)
 
 
@@ -167,7 +173,7 @@ def build_lib(force: bool = False, verbose: bool = False, extra_flags=(), f16: b
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJ, src.replace(".hip", ".o"))
-        if force or _stale(o, [s] + headers):
+        if force or _stale(o, [s] + headers + _ops_headers(src)):
             jobs.append((s, o))
 
     def cc(job):

@@ -9,6 +9,7 @@
 
 #include <vector>
 
+#include "../../include/hiertcn_ops.h"
 #include "common.h"
 #include "exact.h"
 #include "train.h"
@@ -881,6 +882,13 @@ int hiertcn_adam_step(hiertcn_handle_t h, float lr, float beta1, float beta2, fl
   CHECK_READY(h);
   if (!h->train.enabled) return fail(HIERTCN_ERR_STATE, "training is not enabled on this handle");
   HIP_TRY(train_adam(h->m, h->train, lr, beta1, beta2, eps, grad_scale, reinterpret_cast<hipStream_t>(stream)));
+  return HIERTCN_OK;
+}
+
+int hiertcn_train_masters_changed(hiertcn_handle_t h, void* stream) {   // include/hiertcn_ops.h
+  CHECK_READY(h);
+  if (!h->train.enabled) return fail(HIERTCN_ERR_STATE, "training is not enabled on this handle");
+  HIP_TRY(train_refresh_bf16(h->m, h->train, reinterpret_cast<hipStream_t>(stream)));
   return HIERTCN_OK;
 }
 

@@ -1,0 +1,88 @@
+// Shared by the sequence operators (glr.hip, seq_loss.hip, adamw.hip): errors, typed vector access, views.  Unlike the model kernels these take
+// fp32, bfloat16 and IEEE half side by side in both library builds, so nothing here depends on HIERTCN_F16.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/hiertcn_ops.h"
+
+int ops_fail(int code, const char* fmt, ...);   // sets this thread's message, returns code
+#define OPS_TRY(expr)                                                                                                                        \
+  do {                                                                                                                                       \
+    hipError_t e_ = (expr);                                                                                                                  \
+    if (e_ != hipSuccess) return ops_fail(HIERTCN_ERR_HIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__, __LINE__);       \
+  } while (0)
+
+static inline int ops_size(int dtype) { return dtype == HIERTCN_FP32 ? 4 : 2; }
+static inline bool ops_dtype_ok(int dtype) { return dtype >= HIERTCN_FP32 && dtype <= HIERTCN_FP16; }
+
+// A [nb][nt][nd] view with element strides (nd contiguous).  Host side, for the overlap checks.
+struct OpsView {
+  const char* p; int64_t nb, nt, nd, sb, st; int es;
+  int64_t extent() const { return nb && nt && nd ? ((nb - 1) * sb + (nt - 1) * st + nd) * es : 0; }
+};
+static inline OpsView ops_flat(const void* p, int64_t n, int es) { return {static_cast<const char*>(p), 1, 1, n, 0, 0, es}; }
+// rows of the view do not overlap one another (an output may not hold one place twice)
+static inline bool ops_rows_apart(const OpsView& v) {
+  if (v.nb <= 1 && v.nt <= 1) return true;
+  if (v.nb <= 1) return v.st >= v.nd;
+  if (v.nt <= 1) return v.sb >= v.nd;
+  return (v.st >= v.nd && v.sb >= (v.nt - 1) * v.st + v.nd) || (v.sb >= v.nd && v.st >= (v.nb - 1) * v.sb + v.nd);
+}
+// true if the two views may share a place.  Rows of one buffer side by side (the halves of a [B][T][2 D] projection) are told apart.
+static inline bool ops_overlap(const OpsView& a, const OpsView& b) {
+  if (!a.p || !b.p || !a.extent() || !b.extent()) return false;
+  if (a.p + a.extent() <= b.p || b.p + b.extent() <= a.p) return false;
+  const OpsView& lo = a.p <= b.p ? a : b;
+  const OpsView& hi = a.p <= b.p ? b : a;
+  if (a.es != b.es || a.nb != b.nb || a.nt != b.nt || a.nd != b.nd || a.sb != b.sb || a.st != b.st || !ops_rows_apart(a)) return true;
+  // both strides are multiples of the smaller one: two rows are d + k * small apart, nearest for the d % small at hand
+  const int64_t small = (a.nb <= 1 ? a.st : a.nt <= 1 ? a.sb : a.sb < a.st ? a.sb : a.st) * a.es, row = a.nd * a.es;
+  if (small <= 0 || (a.nb > 1 && a.sb * a.es % small) || (a.nt > 1 && a.st * a.es % small)) return true;
+  const int64_t r = (hi.p - lo.p) % small;
+  return !(r >= row && small - r >= row);
+}
+
+// ---- device side ----------------------------------------------------------------------------------------------------------------------------
+template <int VEC>
+struct alignas(4 * VEC) OpsF { float v[VEC]; };
+template <int VEC>
+struct alignas(2 * VEC) OpsH { uint16_t v[VEC]; };
+
+__device__ __forceinline__ float ops_h2f(uint16_t u, int dt) {
+  return dt == HIERTCN_BF16 ? __builtin_bit_cast(float, (uint32_t)u << 16) : (float)__builtin_bit_cast(_Float16, u);
+}
+__device__ __forceinline__ uint16_t ops_f2h(float f, int dt) {   // round to nearest, ties to even
+  if (dt == HIERTCN_BF16) { __bf16 b = (__bf16)f; return __builtin_bit_cast(uint16_t, b); }
+  _Float16 h = (_Float16)f;
+  return __builtin_bit_cast(uint16_t, h);
+}
+// VEC elements of type DT at element offset `off` <-> fp32 registers.  The address is a multiple of VEC elements.
+template <int DT, int VEC>
+__device__ __forceinline__ void ops_ld(const void* __restrict__ p, int64_t off, float (&o)[VEC]) {
+  if constexpr (DT == HIERTCN_FP32) {
+    const OpsF<VEC> x = *reinterpret_cast<const OpsF<VEC>*>(static_cast<const float*>(p) + off);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) o[i] = x.v[i];
+  } else {
+    const OpsH<VEC> x = *reinterpret_cast<const OpsH<VEC>*>(static_cast<const uint16_t*>(p) + off);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) o[i] = ops_h2f(x.v[i], DT);
+  }
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void ops_st(void* __restrict__ p, int64_t off, const float (&o)[VEC]) {
+  if constexpr (DT == HIERTCN_FP32) {
+    OpsF<VEC> x;
+#pragma unroll
+    for (int i = 0; i < VEC; i++) x.v[i] = o[i];
+    *reinterpret_cast<OpsF<VEC>*>(static_cast<float*>(p) + off) = x;
+  } else {
+    OpsH<VEC> x;
+#pragma unroll
+    for (int i = 0; i < VEC; i++) x.v[i] = ops_f2h(o[i], DT);
+    *reinterpret_cast<OpsH<VEC>*>(static_cast<uint16_t*>(p) + off) = x;
+  }
+}
+// 2^x through v_exp_f32 (one ulp); e^x for |x| that matter here
+__device__ __forceinline__ float ops_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }

@@ -1,0 +1,317 @@
+"""CPU side of the sequence operators: the header, the binding and the library agree; bad calls are refused before anything is launched (the
+C entries check shapes, strides, addresses and overlaps on the host, so made-up addresses serve); the oracle's gradients against differences."""
+import ctypes as C
+import os
+import re
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+from hiertcn_amd import _lib, _ops
+from hiertcn_amd._lib import HierTCNError
+from oracle import sequence_oracle as SO
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "hiertcn_ops.h")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(_lib.LIB_PATH):
+        from hiertcn_amd.build import build_lib
+        build_lib()
+    return _ops.lib()
+
+
+def _source():
+    return re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+
+
+def test_header_and_binding_name_the_same_functions(lib):
+    names = set(re.findall(r"\b(hiertcn_[a-z_0-9]+)\s*\(", _source()))
+    assert names == set(_ops.SYMBOLS), names ^ set(_ops.SYMBOLS)
+    for path in (_lib.LIB_PATH, _lib.LIB_PATH_F16):
+        so = C.CDLL(path)
+        assert all(hasattr(so, n) for n in names), path
+    version = int(re.search(r"#define\s+HIERTCN_OPS_VERSION\s+(\d+)", _source()).group(1))
+    assert lib.hiertcn_ops_version() == version == _ops.VERSION
+
+
+def test_struct_layouts(lib, tmp_path):
+    """Field names, offsets and sizes: the header as gcc compiles it, the binding, and the library."""
+    fields = {}
+    for body, name in re.findall(r"typedef\s+struct\s*\{(.*?)\}\s*(hiertcn_\w+_t)\s*;", _source(), flags=re.S):
+        fields[name] = []
+        for decl in body.split(";"):
+            if decl.strip():
+                first, *more = decl.strip().split(",")
+                fields[name] += [re.search(r"(\w+)\s*$", v.strip()).group(1) for v in (first, *more)]
+    by_name = {c.__doc__: c for c in _ops.STRUCTS}
+    assert set(by_name) == set(fields)
+    lines = ["#include <stddef.h>", "#include <stdio.h>", '#include "hiertcn_ops.h"', "int main(void) {"]
+    for st, names in fields.items():
+        lines.append(f'printf("{st} %zu\\n", sizeof({st}));')
+        lines += [f'printf("{st}.{f} %zu\\n", offsetof({st}, {f}));' for f in names]
+    (tmp_path / "l.c").write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-pedantic", "-I", os.path.join(ROOT, "include"), str(tmp_path / "l.c"), "-o", str(tmp_path / "l")], check=True)
+    layout = dict(ln.split() for ln in subprocess.run([str(tmp_path / "l")], check=True, capture_output=True, text=True).stdout.splitlines())
+    for st, cls in by_name.items():
+        assert [f for f, _ in cls._fields_] == fields[st], st
+        assert C.sizeof(cls) == int(layout[st])
+        for f in fields[st]:
+            assert getattr(cls, f).offset == int(layout[f"{st}.{f}"]), (st, f)
+    sizes = (C.c_size_t * len(_ops.STRUCTS))()
+    assert lib.hiertcn_ops_struct_sizes(sizes) == 0 and list(sizes) == [C.sizeof(c) for c in _ops.STRUCTS]
+
+
+# ---- gated linear recurrence ------------------------------------------------------------------------------------------------------------------
+BASE = 1 << 20      # made-up addresses: never dereferenced, the calls below are refused on the host
+
+
+def glr_call(B=2, T=10, D=8, **kw):
+    a = _ops.Glr(B=B, T=T, D=D, dtype=0, cand_act=1)
+    at = BASE
+    for f in ("gate", "cand", "out", "dout", "dgate", "dcand"):
+        setattr(a, f, at)
+        setattr(a, f + "_sb", T * D)
+        setattr(a, f + "_st", D)
+        at += 1 << 20
+    for f in ("state_in", "state_out", "record", "dstate_out", "dstate_in"):
+        setattr(a, f, at)
+        at += 1 << 20
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(B=-1), "negative"), (dict(dtype=5), "dtype"), (dict(cand_act=2), "cand_act"), (dict(gate=None), "null"), (dict(out=None), "null"),
+    (dict(gate_sb=-80), "stride"), (dict(gate=BASE + 2), "multiple"), (dict(state_in=BASE + 1), "multiple"), (dict(out_st=4), "overlap"),
+    (dict(out_sb=0), "overlap"), (dict(out=BASE), "overlaps an input"), (dict(record=BASE + 64), "overlaps an input"),
+    (dict(state_out=BASE + (6 << 20) + 8), "overlaps an input"), (dict(B=1 << 40), "at most"),
+], ids=lambda v: str(v) if isinstance(v, dict) else "")
+def test_glr_forward_refuses(lib, kw, word):
+    a = glr_call(**kw)
+    assert lib.hiertcn_glr_forward(C.byref(a), None) < 0
+    assert word in lib.hiertcn_ops_last_error().decode()
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(dout=None), "null"), (dict(dgate=None), "null"), (dict(record=None), "null"), (dict(dgate=BASE), "overlaps an input"),
+    (dict(dcand=BASE + (4 << 20) + 32), "two outputs"), (dict(dcand_st=7), "overlap"),
+], ids=lambda v: str(v) if isinstance(v, dict) else "")
+def test_glr_backward_refuses(lib, kw, word):
+    a = glr_call(**kw)
+    assert lib.hiertcn_glr_backward(C.byref(a), None) < 0
+    assert word in lib.hiertcn_ops_last_error().decode()
+
+
+def test_glr_a_missing_workspace_is_refused(lib):
+    B, T, D = 1, 100000, 64
+    need = lib.hiertcn_glr_workspace_bytes(B, T, D)
+    assert need > 0 and lib.hiertcn_glr_workspace_bytes(4096, 16, 256) == 0
+    at = 1 << 40
+    a = _ops.Glr(B=B, T=T, D=D, dtype=1, cand_act=0)
+    for f in ("gate", "cand", "out"):
+        setattr(a, f, at)
+        setattr(a, f + "_sb", T * D)
+        setattr(a, f + "_st", D)
+        at += 1 << 32
+    for ws, nbytes in ((None, 0), (at, need - 1), (at + 4, need + 4)):
+        a.workspace, a.workspace_bytes = ws, nbytes
+        assert lib.hiertcn_glr_forward(C.byref(a), None) == -4 and b"workspace" in lib.hiertcn_ops_last_error()
+    assert lib.hiertcn_glr_forward(None, None) == -1
+
+
+def test_glr_python_checks():
+    from hiertcn_amd.glr import glr_scan, glr_step
+    g = torch.zeros(2, 3, 4)
+    with pytest.raises(HierTCNError, match="GPU"):
+        glr_scan(g, g)
+    with pytest.raises(TypeError):
+        glr_scan([1], g)
+    with pytest.raises(HierTCNError, match="dtype"):
+        glr_scan(g.double(), g)
+    with pytest.raises(HierTCNError, match=r"\[B, D\]"):
+        glr_step(g, g, g)
+
+
+def test_glr_oracle_gradients_against_differences():
+    rng = np.random.default_rng(0)
+    B, T, D = 2, 7, 3
+    g, x, dh = (rng.standard_normal((B, T, D)) for _ in range(3))
+    s, ds = rng.standard_normal((B, D)), rng.standard_normal((B, D))
+    mask, lens = (rng.random((B, T)) > 0.3).astype(float), np.array([7, 4])
+    for act in ("tanh", "none"):
+        ref = SO.glr(g, x, s, mask, lens, act, dh, ds)
+        loss = lambda g, x, s: (lambda r: (r["h"] * dh).sum() + (r["state"] * ds).sum())(SO.glr(g, x, s, mask, lens, act))  # noqa: E731
+        for k, (name, v) in enumerate(dict(dgate=g, dcand=x, dstate=s).items()):
+            for i in np.ndindex(v.shape):
+                a, b = [w.copy() for w in (g, x, s)], [w.copy() for w in (g, x, s)]
+                a[k][i] += 1e-6
+                b[k][i] -= 1e-6
+                assert abs((loss(*a) - loss(*b)) / 2e-6 - ref[name][i]) < 1e-8
+
+
+# ---- losses -------------------------------------------------------------------------------------------------------------------------------------
+def rows_call(n=4, T=3, V=50, **kw):
+    r = _ops.Rows(n=n, T=T, V=V, dtype=0, ld=V, dld=V, grad_scale=1.0)
+    at = BASE
+    for f in ("logits", "ids", "logp", "dlogits", "workspace"):
+        setattr(r, f, at)
+        at += 1 << 24
+    r.workspace_bytes = 1 << 22
+    for k, v in kw.items():
+        setattr(r, k, v)
+    return r
+
+
+def outputs(q, names, at=BASE + (8 << 24)):
+    for f in names:
+        setattr(q, f, at)
+        at += 1 << 20
+    return q
+
+
+ROWS_BAD = [(dict(n=0), "at least 1"), (dict(T=0), "at least 1"), (dict(V=0), "at least 1"), (dict(dtype=3), "dtype"), (dict(logits=None), "null"), (dict(ids=None), "null"),
+            (dict(ld=49), "stride"), (dict(dld=10), "stride"), (dict(logits=BASE + 2), "multiple"), (dict(workspace_bytes=8), "workspace"), (dict(workspace=None), "workspace"),
+            (dict(dlogits=BASE + 200), "overlaps"), (dict(logp=BASE + 64), "overlaps"), (dict(workspace=BASE), "overlaps"), (dict(grad_scale=float("inf")), "grad_scale"),
+            (dict(n=1 << 20, T=1 << 20), "at most")]
+
+
+@pytest.mark.parametrize("kw,word", ROWS_BAD, ids=lambda v: str(v) if isinstance(v, dict) else "")
+def test_losses_refuse_bad_rows(lib, kw, word):
+    r = rows_call(**kw)
+    q = outputs(_ops.Preference(kind=0, beta=0.1), ("ref", "loss", "pair_loss", "margin", "seq_logp"))
+    o = outputs(_ops.Policy(clip_low=0.2, clip_high=0.2), ("old_logp", "advantage", "loss", "kl", "clipped"))
+    calls = [lambda: lib.hiertcn_preference_loss(C.byref(r), C.byref(q), None), lambda: lib.hiertcn_policy_loss(C.byref(r), C.byref(o), None)]
+    if not {"dlogits", "dld", "grad_scale"} & set(kw):
+        calls.append(lambda: lib.hiertcn_sequence_logp(C.byref(r), None))
+    for call in calls:
+        assert call() < 0 and word in lib.hiertcn_ops_last_error().decode(), lib.hiertcn_ops_last_error()
+
+
+@pytest.mark.parametrize("kw,word", [(dict(kind=3), "kind"), (dict(beta=0.0), "beta"), (dict(beta=float("nan")), "beta"), (dict(smoothing=0.5), "smoothing"),
+                                     (dict(kind=1, smoothing=0.1), "smoothing"), (dict(ref=None), "ref"), (dict(loss=None), "loss"), (dict(margin=BASE), "overlaps"),
+                                     (dict(seq_logp=BASE + (8 << 24)), "overlaps ref")], ids=str)
+def test_preference_refuses(lib, kw, word):
+    q = outputs(_ops.Preference(kind=0, beta=0.1), ("ref", "loss", "pair_loss", "margin", "seq_logp"))
+    for k, v in kw.items():
+        setattr(q, k, v)
+    assert lib.hiertcn_preference_loss(C.byref(rows_call()), C.byref(q), None) < 0 and word in lib.hiertcn_ops_last_error().decode()
+    assert lib.hiertcn_preference_loss(C.byref(rows_call(n=3)), C.byref(outputs(_ops.Preference(beta=1.0), ("ref", "loss", "pair_loss", "margin", "seq_logp"))), None) < 0
+    assert b"pairs" in lib.hiertcn_ops_last_error()
+
+
+@pytest.mark.parametrize("kw,word", [(dict(mean=2), "mean"), (dict(clip_low=1.5), "clip"), (dict(clip_high=-0.1), "clip"), (dict(kl_coef=0.1), "ref_logp"), (dict(kl_coef=-1.0), "kl_coef"),
+                                     (dict(old_logp=None), "null"), (dict(adv_sn=-1), "stride"), (dict(kl=BASE), "overlaps"), (dict(clipped=BASE + (8 << 24)), "overlaps")], ids=str)
+def test_policy_refuses(lib, kw, word):
+    q = outputs(_ops.Policy(clip_low=0.2, clip_high=0.2, adv_sn=1), ("old_logp", "advantage", "loss", "kl", "clipped"))
+    for k, v in kw.items():
+        setattr(q, k, v)
+    assert lib.hiertcn_policy_loss(C.byref(rows_call()), C.byref(q), None) < 0 and word in lib.hiertcn_ops_last_error().decode(), lib.hiertcn_ops_last_error()
+
+
+def test_loss_python_checks():
+    from hiertcn_amd.sequence_loss import policy_loss, preference_loss, sequence_logp
+    z, ids = torch.zeros(2, 3, 4), torch.zeros(2, 3, dtype=torch.int32)
+    for call in (lambda: sequence_logp(z, ids), lambda: preference_loss(z, ids, torch.zeros(2)), lambda: policy_loss(z, ids, torch.zeros(2, 3), torch.zeros(2))):
+        with pytest.raises(HierTCNError, match="GPU"):
+            call()
+    with pytest.raises(HierTCNError, match="kind"):
+        preference_loss(z, ids, torch.zeros(2), kind="other")
+    with pytest.raises(HierTCNError, match="mean"):
+        policy_loss(z, ids, torch.zeros(2, 3), torch.zeros(2), mean="other")
+
+
+def test_loss_oracle_gradients_against_differences():
+    rng = np.random.default_rng(3)
+    n, T, V = 4, 3, 6
+    z = 2 * rng.standard_normal((n, T, V))
+    ids = rng.integers(0, V, (n, T))
+    lp = SO.rows(z, ids)["logp"]
+    old, ref, adv, sref = lp + rng.choice([-0.5, 0.1, 0.4], (n, T)), lp + 0.3 * rng.standard_normal((n, T)), rng.standard_normal(n), rng.standard_normal(n)
+    forms = [lambda x, m=m: SO.policy(x, ids, old, adv, ref, 0.2, 0.3, 0.1, m, 2.0) for m in ("sequence", "token")]
+    forms += [lambda x, k=k, a=a: SO.preference(x, ids, sref, 0.4, k, 0.1 if k == "sigmoid" else 0.0, a, 2.0) for k in ("sigmoid", "hinge", "squared") for a in (False, True)]
+    for form in forms:
+        d = form(z)["dlogits"]
+        for i in np.ndindex(z.shape):
+            a, b = z.copy(), z.copy()
+            a[i] += 1e-6
+            b[i] -= 1e-6
+            assert abs(2.0 * (form(a)["loss"] - form(b)["loss"]) / 2e-6 - d[i]) < 1e-7 * max(1, abs(d).max())
+
+
+# ---- AdamW -----------------------------------------------------------------------------------------------------------------------------------------
+def adamw_call(**kw):
+    t = _ops.AdamwTensor(numel=1000, grad_dtype=0, copy_dtype=1, index=0)
+    at = BASE
+    for f in ("param", "grad", "copy", "m", "v", "m_scale", "v_scale"):
+        setattr(t, f, at)
+        at += 1 << 20
+    a = _ops.Adamw(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, t=1, state_bits=8)
+    for k, v in kw.items():
+        setattr(t if hasattr(t, k) else a, k, v)
+    return t, a
+
+
+@pytest.mark.parametrize("kw,word", [(dict(state_bits=16), "state_bits"), (dict(t=0), "from 1"), (dict(beta1=1.0), "betas"), (dict(lr=float("nan")), "lr"), (dict(eps=-1.0), "eps"),
+                                     (dict(grad_scale=float("inf")), "grad_scale"), (dict(numel=-1), "elements"), (dict(param=None), "null"), (dict(v_scale=None), "null"),
+                                     (dict(grad_dtype=7), "gradient dtype"), (dict(copy_dtype=0), "copy dtype"), (dict(weight_decay=-0.1), "weight_decay"),
+                                     (dict(param=BASE + 2), "multiple"), (dict(m=BASE), "overlap"), (dict(grad=BASE + 400), "overlap")], ids=str)
+def test_adamw_refuses(lib, kw, word):
+    t, a = adamw_call(**kw)
+    assert lib.hiertcn_adamw_step(C.byref(t), 1, C.byref(a), None) < 0 and word in lib.hiertcn_ops_last_error().decode(), lib.hiertcn_ops_last_error()
+
+
+def test_adamw_moments_refuses(lib):
+    t, _ = adamw_call()
+    for m, v, word in ((BASE + (3 << 20), None, "overlaps a state"), (BASE + (9 << 20), BASE + (9 << 20) + 64, "outputs overlap"), (BASE + 1, None, "multiple")):
+        mo, vo = (C.c_void_p * 1)(m), (C.c_void_p * 1)(v)
+        assert lib.hiertcn_adamw_moments(C.byref(t), 1, mo, vo, None) < 0 and word in lib.hiertcn_ops_last_error().decode()
+
+
+def test_adamw_python_checks():
+    from hiertcn_amd.adamw import AdamW
+    with pytest.raises(HierTCNError, match="no parameters"):
+        AdamW([])
+    with pytest.raises(HierTCNError, match="state_bits"):
+        AdamW([torch.zeros(3)], state_bits=4)
+    with pytest.raises(HierTCNError, match="GPU"):
+        AdamW([torch.zeros(3)])
+
+
+def test_random_bits_are_even():
+    """The rounding's bits: every bit of neighbouring elements, steps and tensors is one half the time (2^16 samples: 5 sigma = 0.01), and bits of one element and the
+    next, of one step and the next, agree half the time."""
+    n = 1 << 16
+    base = SO.mix(n, 3, 10, 12345)
+    bit = lambda x: (x[:, None] >> np.arange(32, dtype=np.uint32)) & 1  # noqa: E731
+    for other in (SO.mix(n, 3, 11, 12345), SO.mix(n, 4, 10, 12345), SO.mix(n, 3, 10, 12346), np.roll(base, 1)):
+        assert abs(bit(other).mean(0) - 0.5).max() < 0.01
+        assert abs((bit(other) == bit(base)).mean(0) - 0.5).max() < 0.01
+
+
+def test_codes_keep_the_expectation_and_nearest_would_not():
+    """Mean of the decoded value over all 65,536 random numbers = the value (to the code width / 65,536 and fp32); and why it has to: v under a constant gradient."""
+    rng = np.random.default_rng(4)
+    for squared in (False, True):
+        mag = np.abs(rng.standard_normal(256)).astype(np.float32) + np.float32(1e-3)
+        want = mag.astype(np.float64) ** (2 if squared else 1)
+        total = np.zeros(256)
+        for u in range(0, 65536, 64):
+            code, scale = SO.encode(mag, np.full(256, u + 31, np.uint32), squared)
+            total += SO.decode(code.astype(np.uint8), scale, squared)
+        got = total / 1024
+        width = 4 if squared else 2
+        assert (np.abs(got - want) <= want.max() * (width / 255 / 1024 + 1e-6) + 1e-5 * want).all()
+    v, b2 = np.full(256, 0.25, np.float32), 0.999      # held as sqrt(v) = 0.5; the gradient's size is 1 from now on
+    v[0] = 1.0
+    q, s = SO.encode(np.sqrt(v), np.full(256, 1 << 15, np.uint32), True)
+    q0 = q.copy()
+    for _ in range(200):
+        v = (SO.decode(q.astype(np.uint8), s, True) * b2 + (1 - b2)).astype(np.float32)
+        q, s = SO.encode(np.sqrt(v), np.full(256, 1 << 15, np.uint32), True)
+    assert (q == q0).all(), "rounding to nearest: two hundred steps do not move a code"
