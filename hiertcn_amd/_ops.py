@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -103,6 +104,8 @@ def check(rc: int):
 
 def need(t, name, dtype, device, shape, contiguous=True):
     """The argument check of the operators: type, place, element type, shape and layout of a tensor."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == shape and (not contiguous or t.is_contiguous()):
+        return t
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype != dtype:
@@ -111,9 +114,7 @@ def need(t, name, dtype, device, shape, contiguous=True):
         raise HierTCNError(f"{name}: on {t.device}, expected {device}")
     if t.shape != shape:
         raise HierTCNError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if contiguous and not t.is_contiguous():
-        raise HierTCNError(f"{name}: must be contiguous")
-    return t
+    raise HierTCNError(f"{name}: must be contiguous")
 
 
 def on_gpu(t, name):
@@ -129,11 +130,20 @@ def on_gpu(t, name):
 
 def call(fn, device, *args):
     """fn(*args, stream) on `device` and its current stream, whatever the current device is."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))     # (torch.cuda.current_stream(device).cuda_stream without building the Stream object)
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        check(rc)
+
+
+@functools.lru_cache(maxsize=4096)
+def size(name, *dims):
+    """A workspace or record size of the library: a function of the dimensions alone."""
+    return getattr(lib(), name)(*dims)
 
 
 def workspace(nbytes, device):

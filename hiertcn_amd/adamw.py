@@ -42,6 +42,7 @@ class AdamW:
         self.lr, self.betas, self.eps, self.state_bits, self.seed, self.t = float(lr), (float(betas[0]), float(betas[1])), float(eps), state_bits, int(seed), 0
         self.weight_decay, self.copies = decay, copies
         self._desc = (_ops.AdamwTensor * n)()
+        self._flat = [torch.Size([p.numel()]) for p in self.params]
         for i, (p, c, d) in enumerate(zip(self.params, copies, self._desc)):
             d.numel, d.param, d.weight_decay, d.index = p.numel(), p.data_ptr(), decay[i], i
             if c is not None:
@@ -145,12 +146,6 @@ class AdamW:
             out = tuple([torch.empty(p.numel(), dtype=torch.float32, device=self.device) for p in self.params] for _ in range(2))
         if len(out[0]) != n or len(out[1]) != n:
             raise HierTCNError(f"{n} parameters, outputs for {len(out[0])} and {len(out[1])}")
-        ptrs = []
-        for name, lst in zip("mv", out):
-            arr = (C.c_void_p * n)()
-            for i, (o, p) in enumerate(zip(lst, self.params)):
-                if o is not None:
-                    arr[i] = need(o, f"out {name}[{i}]", torch.float32, self.device, torch.Size([p.numel()])).data_ptr()
-            ptrs.append(arr)
+        ptrs = [(C.c_void_p * n)(*[None if o is None else need(o, "out", torch.float32, self.device, k).data_ptr() for o, k in zip(lst, self._flat)]) for lst in out]
         _ops.call(_ops.lib().hiertcn_adamw_moments, self.device, self._desc, n, *ptrs)
         return out

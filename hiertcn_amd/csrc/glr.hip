@@ -2,45 +2,57 @@
 // the update of customed_gru_cell.py:309-337 with gates that do not read the state, hence a scan.
 //
 // The map of a run of steps is h -> A h + S (A the product of the a_t = u_t keep_t, S the run's own state from zero), and maps compose:
-// (A2, S2) after (A1, S1) is (A2 A1, A2 S1 + S2).  Time is cut into SEGMENTS of 8 steps; a thread owns a segment of VEC neighbouring channels and
-// keeps its a_t and (1 - u_t) c_t in registers, so that gate and cand are read once: it forms (A, S), learns the state before its segment from the maps
-// of the segments before it (lanes of a wave by shuffles, waves of a workgroup through LDS, earlier tiles as a carry in registers, earlier
-// workgroups through `agg`), and replays the segment from there.
+// (A2, S2) after (A1, S1) is (A2 A1, A2 S1 + S2).  Time is cut into SEGMENTS of 16 steps.  A wave owns a segment of 64 VEC neighbouring channels of one
+// sequence, so that everything but the channels -- rows, masks, lengths, branches -- is uniform over it and lives in scalar registers.  It keeps its
+// a_t and (1 - u_t) c_t in vector registers, so that gate and cand are read once: it forms (A, S), learns the state before its segment from the
+// maps of the segments before it (waves of the workgroup, a TILE, through LDS; earlier tiles as a carry in registers), and replays the segment from there.
+//
+// Where there are few sequences for the machine the tiles of a sequence go to different workgroups (CHAIN).  A workgroup publishes its tile's map, applies
+// those of the tiles before it in its group of 16 to the state before the group, and the last of a group publishes the state behind it.  The order of
+// all that is the order of time, whoever waits for whom, so results do not depend on timing.  A word (A, S) is its own flag: 64 bits, written by one store that
+// goes past the L2s, all ones until then (a NaN is stored as the canonical one, so that no result looks like that).  A workgroup waits for workgroups of lower
+// TICKETS only, tickets are drawn at the start of a workgroup, and the one with the lowest ticket waits for nobody: every wait ends.
 //
 // The backward pass is the same recurrence the other way round, lambda_t = dout_t + a_{t+1} lambda_{t+1}: with r_t = a_t lambda_t a run maps r -> A r + Q
-// with the same A.  States are not read back from the rounded output: the forward pass leaves the fp32 state before every segment in `record`, 1/8 of
-// a [B][T][D] fp32 array, and a thread replays its segment from there.
+// with the same A.  States are not read back from the rounded output: the forward pass leaves the fp32 state before every segment in `record`, 1/16 of
+// a [B][T][D] fp32 array, and a wave replays its segment from there.
 //
-// A reset has to cut a state that is NaN or infinite (0 * NaN = NaN), and nothing else may: A is exactly 0 only where a reset lies in the run (the
-// product of the gates alone is kept from underflowing to 0), and a map with A = 0 ignores what it is applied to.
+// A reset has to cut a state that is NaN or infinite (0 * NaN = NaN), and nothing else may: with a mask, A is exactly 0 only where a reset lies in the run
+// (the product of the gates alone is kept from underflowing to 0), and a map with A = 0 ignores what it is applied to.  Without one maps are plain fma's.
 #include "ops.h"
 
 namespace {
 
-constexpr int SEG = 8;           // steps of a segment = distance of the records
-constexpr int CB = 64;           // channels of a workgroup
+constexpr int SEG = 16;          // steps of a segment = distance of the records
+constexpr int MAXW = 16;         // waves of a workgroup, at most
 constexpr float TINY = 1.401298464e-45f;
 
 struct GlrP {
   hiertcn_glr_t a;
-  int64_t nseg;                  // ceil(T / SEG)
+  int nseg;                      // ceil(T / SEG)
   int ncb;                       // channel blocks
-  int nchunk, chunk_tiles;       // the time axis over several workgroups
-  float2* agg;                   // [nchunk][B][D]: the chunks' maps
-  float* state0;                 // [B][D] copy of state_in (state_out may be state_in) when nchunk > 1
+  // CHAIN
+  int ntile;                     // tiles of a sequence, each a workgroup
+  uint64_t* map;                 // [ntile][B][D]: the tiles' maps
+  uint64_t* behind;              // [ntile / GROUP][B][D]: the state behind a group, in the low half
+  float* state0;                 // [B][D]: the state before the first tile (state_out may be state_in)
+  unsigned* ticket;
 };
+constexpr int GROUP = 16;        // tiles of a group
+constexpr uint64_t NOTHING = ~0ull;
 
-struct Map { float A, S; };
-__device__ __forceinline__ float map_a(float A1, float A2) { return A1 == 0.f || A2 == 0.f ? 0.f : fmaxf(A1 * A2, TINY); }
-__device__ __forceinline__ float map_s(float A2, float S1, float S2) { return A2 == 0.f ? S2 : fmaf(A2, S1, S2); }
+// maps: composition and application.  CUT: A = 0 marks a reset
+template <bool CUT>
+__device__ __forceinline__ float map_a(float A1, float A2) { return !CUT ? A1 * A2 : A1 == 0.f || A2 == 0.f ? 0.f : fmaxf(A1 * A2, TINY); }
+template <bool CUT>
+__device__ __forceinline__ float map_s(float A2, float S1, float S2) { return CUT && A2 == 0.f ? S2 : fmaf(A2, S1, S2); }
 
 // u = sigmoid(g) and w = 1 - u = sigmoid(-g), each to a few ulp (1 - u formed from u would lose the small ones)
 __device__ __forceinline__ void gate_of(float g, float& u, float& w) {
   const float e = ops_exp(-fabsf(g));
-  const float r = __builtin_amdgcn_rcpf(1.f + e);
-  u = g >= 0.f ? r : e * r;
-  w = g >= 0.f ? e * r : r;
-  if (g != g) u = w = g;
+  const float r = __builtin_amdgcn_rcpf(1.f + e), er = e * r;
+  u = g >= 0.f ? r : er;
+  w = g >= 0.f ? er : r;
 }
 // tanh to a few ulp: the odd series where (1 - e^-2x) / (1 + e^-2x) would cancel
 __device__ __forceinline__ float tanh_of(float x) {
@@ -54,429 +66,435 @@ __device__ __forceinline__ float tanh_of(float x) {
   return a < 0.3f ? fmaf(x * x2, s, x) : big;
 }
 
-// what a thread knows of its place
+__device__ __forceinline__ int clamped(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+// steps of a sequence that count, as a scalar (a load through a pointer that the outputs might alias is not one by itself)
+__device__ __forceinline__ int length_of(const hiertcn_glr_t& a, int64_t b) {
+  return __builtin_amdgcn_readfirstlane(a.lengths ? clamped(a.lengths[b], 0, (int)a.T) : (int)a.T);
+}
+
+// The mask of the steps t0 .. t0 + n - 1 (n >= 1), one to a lane; and the uniform word whose bit j says whether step t0 + j keeps the state (steps behind the end do)
+template <bool CUT>
+__device__ __forceinline__ float load_mask(const hiertcn_glr_t& a, int64_t b, int t0, int n) {
+  const int lane = threadIdx.x & 63;
+  return CUT ? a.mask[b * a.mask_sb + (t0 + (lane < n ? lane : n - 1)) * a.mask_st] : 1.f;
+}
+template <bool CUT>
+__device__ __forceinline__ uint32_t keep_bits(float mask, int n) {
+  return CUT ? ~(uint32_t)__ballot((int)(threadIdx.x & 63) < n && mask == 0.f) : 0xffffffffu;
+}
+// x, or 0 where bit j of the (uniform) word is clear: an AND with 0 or all ones, which takes NaN and infinity too
+template <bool CUT>
+__device__ __forceinline__ float held(float x, uint32_t keep, int j) {
+  return CUT ? __builtin_bit_cast(float, __builtin_bit_cast(int, x) & __builtin_amdgcn_sbfe((int)keep, j, 1)) : x;
+}
+// The word again, opaque to the optimiser: the 16 masks that it stands for are formed anew in every loop instead of living in scalar registers throughout.
+__device__ __forceinline__ uint32_t anew(uint32_t keep) {
+  asm volatile("" : "+s"(keep));
+  return keep;
+}
+// A wave's place: everything here but `off` and `chan` is uniform.
 template <int VEC>
 struct Place {
-  static constexpr int CL = CB / VEC, TS = 64 / CL;
-  int64_t b, ch;                 // lane (sequence) and first channel
-  bool chan;                     // the channels exist
-  int len;                       // steps of the sequence that count
+  int w, nw, off;                // wave of the workgroup, waves; this lane's first channel of the block
+  int tile;                      // CHAIN's, in the order of the tickets
+  int64_t b, ch0;
+  bool chan;
+  __device__ Place(const GlrP& p, unsigned blk) {
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    nw = blockDim.x >> 6;
+    const unsigned per = (unsigned)p.ncb * (unsigned)p.a.B;      // (the grid fits 31 bits)
+    tile = blk / per;
+    const unsigned rest = blk % per;
+    b = rest / (unsigned)p.ncb;
+    ch0 = (int64_t)(rest % (unsigned)p.ncb) * 64 * VEC;
+    off = (threadIdx.x & 63) * VEC;
+    chan = ch0 + off < p.a.D;
+    if (!chan) off = 0;
+  }
 };
-
-__device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
-__device__ __forceinline__ int64_t length_of(const hiertcn_glr_t& a, int64_t b) { return a.lengths ? clamp64(a.lengths[b], 0, a.T) : a.T; }
-
-// bits of the steps t0 .. t0 + n - 1 whose state is kept (steps behind the end keep it)
-__device__ __forceinline__ uint32_t keep_bits(const hiertcn_glr_t& a, int64_t b, int64_t t0, int n) {
-  uint32_t k = 0xffffffffu;
-  if (a.mask) {
-    const float* m = a.mask + b * a.mask_sb + t0 * a.mask_st;
-    for (int j = 0; j < n; j++)
-      if (m[j * a.mask_st] == 0.f) k &= ~(1u << j);
-  }
-  return k;
-}
-
-// Loads the gates (and candidates) of a segment with n >= 1 live steps; a dead step repeats the last live one's address.
-template <int DT, int VEC>
-__device__ __forceinline__ void load_rows(const void* p, int64_t base, int64_t st, int n, float (&o)[SEG][VEC]) {
-  if (__all(n == SEG)) {
-#pragma unroll
-    for (int j = 0; j < SEG; j++) ops_ld<DT, VEC>(p, base + j * st, o[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < SEG; j++) ops_ld<DT, VEC>(p, base + (j < n ? j : n - 1) * st, o[j]);
-  }
-}
-
-// a_t and b_t = w_t c_t of a segment (identity steps behind n)
-template <int DT, int VEC, bool TANH>
-__device__ __forceinline__ void load_forward(const hiertcn_glr_t& a, int64_t b, int64_t t0, int64_t ch, int n, float (&u)[SEG][VEC], float (&s)[SEG][VEC]) {
-  if (n > 0) {
-    load_rows<DT, VEC>(a.gate, b * a.gate_sb + t0 * a.gate_st + ch, a.gate_st, n, u);
-    load_rows<DT, VEC>(a.cand, b * a.cand_sb + t0 * a.cand_st + ch, a.cand_st, n, s);
-  }
-#pragma unroll
-  for (int j = 0; j < SEG; j++)
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      if (j < n) {
-        float w;
-        gate_of(u[j][i], u[j][i], w);
-        s[j][i] = w * (TANH ? tanh_of(s[j][i]) : s[j][i]);
-      } else {
-        u[j][i] = 1.f;
-        s[j][i] = 0.f;
-      }
-    }
-}
+// a [.][D] fp32 row of states
 template <int VEC>
-__device__ __forceinline__ void segment_map(const float (&u)[SEG][VEC], const float (&s)[SEG][VEC], uint32_t keep, float (&A)[VEC], float (&S)[VEC]) {
-#pragma unroll
-  for (int i = 0; i < VEC; i++) A[i] = 1.f, S[i] = 0.f;
-#pragma unroll
-  for (int j = 0; j < SEG; j++)
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      S[i] = keep >> j & 1 ? fmaf(u[j][i], S[i], s[j][i]) : s[j][i];
-      A[i] *= u[j][i];
-    }
-#pragma unroll
-  for (int i = 0; i < VEC; i++) A[i] = keep == 0xffffffffu ? (A[i] == A[i] ? fmaxf(A[i], TINY) : A[i]) : 0.f;
-}
-// replays a segment from the state h, writing nrow output rows
-template <int DT, int VEC>
-__device__ __forceinline__ void replay(const hiertcn_glr_t& a, int64_t b, int64_t t0, int64_t ch, bool chan, int n, int nrow, uint32_t keep, const float (&u)[SEG][VEC],
-                                       const float (&s)[SEG][VEC], float (&h)[VEC]) {
-  const int64_t base = b * a.out_sb + t0 * a.out_st + ch;
-#pragma unroll
-  for (int j = 0; j < SEG; j++) {
-    float o[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      h[i] = keep >> j & 1 ? fmaf(u[j][i], h[i], s[j][i]) : s[j][i];
-      o[i] = j < n ? h[i] : 0.f;
-    }
-    if (j < nrow && chan) ops_st<DT, VEC>(a.out, base + j * a.out_st, o);
-  }
-}
-template <int VEC>
-__device__ __forceinline__ void get_state(const float* p, int64_t b, int64_t D, int64_t ch, float (&h)[VEC]) {
-  if (p) ops_ld<HIERTCN_FP32, VEC>(p, b * D + ch, h);
+__device__ __forceinline__ void get_state(const float* p, int64_t row, const Place<VEC>& at, float (&h)[VEC]) {
+  if (p) ops_ld<HIERTCN_FP32, VEC>(p + row, at.off, h);
   else
 #pragma unroll
     for (int i = 0; i < VEC; i++) h[i] = 0.f;
 }
-
-// ---- forward, one thread a sequence's channels, segment after segment: many lanes, or few steps --------------------------------------------------
-template <int DT, int VEC, bool TANH>
-__global__ __launch_bounds__(64) void k_glr_seq(GlrP p) {
-  const hiertcn_glr_t& a = p.a;
-  const int64_t groups = a.D / VEC, id = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (id >= a.B * groups) return;
-  const int64_t b = id / groups, ch = id % groups * VEC;
-  const int64_t len = length_of(a, b);
-  float h[VEC], u[SEG][VEC], s[SEG][VEC];
-  get_state<VEC>(a.state_in, b, a.D, ch, h);
-  for (int64_t g = 0; g < p.nseg; g++) {
-    const int64_t t0 = g * SEG;
-    const int n = (int)clamp64(len - t0, 0, SEG), nrow = (int)clamp64(a.T - t0, 0, SEG);
-    if (a.record) ops_st<HIERTCN_FP32, VEC>(a.record, (b * p.nseg + g) * a.D + ch, h);
-    load_forward<DT, VEC, TANH>(a, b, t0, ch, n, u, s);
-    const uint32_t keep = keep_bits(a, b, t0, n);
-    replay<DT, VEC>(a, b, t0, ch, true, n, nrow, keep, u, s, h);
-  }
-  if (a.state_out) ops_st<HIERTCN_FP32, VEC>(a.state_out, b * a.D + ch, h);
+template <int VEC>
+__device__ __forceinline__ void put_state(float* p, int64_t row, const Place<VEC>& at, const float (&h)[VEC]) {
+  if (at.chan) ops_st<HIERTCN_FP32, VEC>(p + row, at.off, h);
 }
+template <int DT>
+__device__ __forceinline__ const char* row_ptr(const void* p, int64_t off) { return static_cast<const char*>(p) + off * (DT == HIERTCN_FP32 ? 4 : 2); }
 
-// ---- the maps of a workgroup's segments ---------------------------------------------------------------------------------------------------------
-// In: this thread's map.  Out: the state before (REV: behind) its segment, given `carry` before the tile, and `carry` behind it.  One barrier; `lds`
-// alternates between two buffers, so that the next tile's writes need no second one.
-template <int VEC, bool REV>
-__device__ __forceinline__ void tile_scan(float2* lds, int nw, int w, int ts, int cl, const float (&A)[VEC], const float (&S)[VEC], float (&carry)[VEC], float (&h)[VEC]) {
-  constexpr int CL = CB / VEC, TS = 64 / CL;
-  const int order = REV ? TS - 1 - ts : ts;
-  float IA[VEC], IS[VEC];          // the maps of the wave's segments up to and with this one
+// The n >= 1 live rows of a segment; a dead step reads the last live row again (no branches: all loads are in flight together).
+template <int DT, int VEC>
+__device__ __forceinline__ void load_rows(const void* p, int64_t base, int64_t st, int off, int n, typename OpsRaw<DT, VEC>::type (&o)[SEG]) {
+  const char* q = row_ptr<DT>(p, base);
 #pragma unroll
-  for (int i = 0; i < VEC; i++) IA[i] = A[i], IS[i] = S[i];
-#pragma unroll
-  for (int d = 1; d < TS; d <<= 1)
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      const float pa = REV ? __shfl_down(IA[i], d * CL) : __shfl_up(IA[i], d * CL), ps = REV ? __shfl_down(IS[i], d * CL) : __shfl_up(IS[i], d * CL);
-      if (order >= d) {
-        IS[i] = map_s(IA[i], ps, IS[i]);
-        IA[i] = map_a(pa, IA[i]);
-      }
-    }
-  if (order == TS - 1)
-#pragma unroll
-    for (int i = 0; i < VEC; i++) lds[w * CB + cl * VEC + i] = make_float2(IA[i], IS[i]);
-  float XA[VEC], XS[VEC];          // ... before this one
-#pragma unroll
-  for (int i = 0; i < VEC; i++) {
-    const float pa = REV ? __shfl_down(IA[i], CL) : __shfl_up(IA[i], CL), ps = REV ? __shfl_down(IS[i], CL) : __shfl_up(IS[i], CL);
-    XA[i] = order ? pa : 1.f;
-    XS[i] = order ? ps : 0.f;
-  }
-  __syncthreads();
-  for (int q = 0; q < nw; q++) {
-    const int ww = REV ? nw - 1 - q : q;
-    if (ww == w)
-#pragma unroll
-      for (int i = 0; i < VEC; i++) h[i] = map_s(XA[i], carry[i], XS[i]);
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      const float2 m = lds[ww * CB + cl * VEC + i];
-      carry[i] = map_s(m.x, carry[i], m.y);
-    }
+  for (int j = 0; j < SEG; j++) {
+    o[j] = reinterpret_cast<const typename OpsRaw<DT, VEC>::type*>(q)[off / VEC];
+    q = row_ptr<DT>(q, j + 1 < n ? st : 0);
   }
 }
 
-// ---- forward, a workgroup 64 channels of a sequence and a tile of nw * TS segments at a time --------------------------------------------------------
-// AGG: only the map of the chunk is wanted (first pass of a time axis that is cut over workgroups).
-template <int DT, int VEC, bool TANH, bool AGG>
-__global__ __launch_bounds__(1024) void k_glr_tile(GlrP p) {
-  constexpr int CL = CB / VEC, TS = 64 / CL;
-  __shared__ float2 lds[2][16 * CB];
-  const hiertcn_glr_t& a = p.a;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, ts = lane / CL, cl = lane % CL;
-  const int64_t blk = blockIdx.x, cb = blk % p.ncb, b = blk / p.ncb % a.B, chunk = blk / p.ncb / a.B;
-  const bool chan = cb * CB + cl * VEC < a.D;
-  const int64_t ch = chan ? cb * CB + cl * VEC : 0;
-  const int64_t len = length_of(a, b);
-  const int tile_seg = nw * TS;
-  const int64_t seg0 = chunk * p.chunk_tiles * tile_seg;
-  const int64_t seg1 = p.nchunk > 1 && chunk + 1 < p.nchunk ? seg0 + (int64_t)p.chunk_tiles * tile_seg : p.nseg;
-  float carry[VEC], carryA[VEC], h[VEC], u[SEG][VEC], s[SEG][VEC], A[VEC], S[VEC];
-  if (AGG) {
+// the first nrow rows of a segment
+template <int DT, int VEC>
+__device__ __forceinline__ void store_rows(const char* q, int64_t st, const Place<VEC>& at, int nrow, const float (&o)[SEG][VEC]) {
+  if (nrow == SEG) {
+    if (at.chan)
 #pragma unroll
-    for (int i = 0; i < VEC; i++) carry[i] = 0.f, carryA[i] = 1.f;
-    if (chunk == 0 && w == 0 && ts == 0 && chan) {
-      get_state<VEC>(a.state_in, b, a.D, ch, h);
-      ops_st<HIERTCN_FP32, VEC>(p.state0, b * a.D + ch, h);
-    }
-  } else if (p.nchunk > 1) {
-    get_state<VEC>(p.state0, b, a.D, ch, carry);
-    for (int64_t q = 0; q < chunk; q++)
+      for (int j = 0; j < SEG; j++, q = row_ptr<DT>(q, st)) ops_st<DT, VEC>(const_cast<char*>(q), at.off, o[j]);
+  } else if (at.chan) {
+#pragma unroll
+    for (int j = 0; j < SEG; j++, q = row_ptr<DT>(q, st))
+      if (j < nrow) ops_st<DT, VEC>(const_cast<char*>(q), at.off, o[j]);
+  }
+}
+
+// the product of a segment's gates as the A of its map
+template <int VEC, bool CUT>
+__device__ __forceinline__ void close_map(uint32_t keep, float (&A)[VEC]) {
+  if (CUT)
+#pragma unroll
+    for (int i = 0; i < VEC; i++) A[i] = keep == 0xffffffffu ? (A[i] == A[i] ? fmaxf(A[i], TINY) : A[i]) : 0.f;
+}
+
+// The state before (REV: behind) every wave's segment, given `carry` before the tile; `carry` behind it.  One barrier; `lds` alternates between two buffers, so
+// that the next tile's writes need no second one.
+template <int VEC>
+__device__ __forceinline__ void put_map(float2* lds, const Place<VEC>& at, const float (&A)[VEC], const float (&S)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; i++) lds[(at.w * VEC + i) * 64 + (threadIdx.x & 63)] = make_float2(A[i], S[i]);
+}
+// folds the maps of the waves onto `carry`, in the order of time; h: before this wave's
+template <int VEC, bool CUT, bool REV>
+__device__ __forceinline__ void fold_waves(const float2* lds, const Place<VEC>& at, float (&carry)[VEC], float (&h)[VEC]) {
+  const int lane = threadIdx.x & 63;
+  for (int q0 = 0; q0 < at.nw; q0 += 4) {
+    float2 m[4][VEC];
+#pragma unroll
+    for (int k = 0; k < 4; k++)
 #pragma unroll
       for (int i = 0; i < VEC; i++) {
-        const float2 m = p.agg[(q * a.B + b) * a.D + ch + i];
-        carry[i] = map_s(m.x, carry[i], m.y);
+        const int q = q0 + k < at.nw ? q0 + k : at.nw - 1;
+        m[k][i] = lds[((REV ? at.nw - 1 - q : q) * VEC + i) * 64 + lane];
       }
-  } else {
-    get_state<VEC>(a.state_in, b, a.D, ch, carry);
-  }
-  int turn = 0;
-  for (int64_t g0 = seg0; g0 < seg1; g0 += tile_seg, turn ^= 1) {
-    const int64_t g = g0 + w * TS + ts, t0 = g * SEG;
-    const int n = (int)clamp64(len - t0, 0, SEG), nrow = g < seg1 ? (int)clamp64(a.T - t0, 0, SEG) : 0;
-    if (AGG && g0 * SEG >= len) break;       // (len is the workgroup's)
-    load_forward<DT, VEC, TANH>(a, b, t0, ch, n, u, s);
-    const uint32_t keep = keep_bits(a, b, t0, n);
-    segment_map<VEC>(u, s, keep, A, S);
-    if (AGG) {
 #pragma unroll
-      for (int i = 0; i < VEC; i++) h[i] = A[i];
-      float before[VEC];
-      tile_scan<VEC, false>(lds[turn], nw, w, ts, cl, A, S, carry, before);
-      for (int q = 0; q < nw; q++)
+    for (int k = 0; k < 4; k++) {
+      if (q0 + k >= at.nw) break;
+      if ((REV ? at.nw - 1 - (q0 + k) : q0 + k) == at.w)
 #pragma unroll
-        for (int i = 0; i < VEC; i++) carryA[i] = map_a(carryA[i], lds[turn][q * CB + cl * VEC + i].x);
-      continue;
+        for (int i = 0; i < VEC; i++) h[i] = carry[i];
+#pragma unroll
+      for (int i = 0; i < VEC; i++) carry[i] = map_s<CUT>(m[k][i].x, carry[i], m[k][i].y);
     }
-    tile_scan<VEC, false>(lds[turn], nw, w, ts, cl, A, S, carry, h);
-    if (a.record && nrow > 0 && chan) ops_st<HIERTCN_FP32, VEC>(a.record, (b * p.nseg + g) * a.D + ch, h);
-    replay<DT, VEC>(a, b, t0, ch, chan, n, nrow, keep, u, s, h);
   }
-  if (w != 0 || ts != 0 || !chan) return;
-  if (AGG) {
+}
+template <int VEC, bool CUT, bool REV>
+__device__ __forceinline__ void tile_scan(float2* lds, const Place<VEC>& at, const float (&A)[VEC], const float (&S)[VEC], float (&carry)[VEC], float (&h)[VEC]) {
+  if (at.nw == 1) {
 #pragma unroll
-    for (int i = 0; i < VEC; i++) p.agg[(chunk * a.B + b) * a.D + ch + i] = make_float2(carryA[i], carry[i]);
-  } else if (a.state_out && chunk == p.nchunk - 1) {
-    ops_st<HIERTCN_FP32, VEC>(a.state_out, b * a.D + ch, carry);
+    for (int i = 0; i < VEC; i++) {
+      h[i] = carry[i];
+      carry[i] = map_s<CUT>(A[i], carry[i], S[i]);
+    }
+    return;
   }
+  put_map<VEC>(lds, at, A, S);
+  __syncthreads();
+  fold_waves<VEC, CUT, REV>(lds, at, carry, h);
+}
+
+// ---- CHAIN ------------------------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t word(float lo, float hi) {
+  if (lo != lo) lo = __builtin_bit_cast(float, 0x7fc00000u);
+  return (uint64_t)__builtin_bit_cast(uint32_t, hi) << 32 | __builtin_bit_cast(uint32_t, lo);
+}
+__device__ __forceinline__ float low(uint64_t v) { return __builtin_bit_cast(float, (uint32_t)v); }
+__device__ __forceinline__ float high(uint64_t v) { return __builtin_bit_cast(float, (uint32_t)(v >> 32)); }
+__device__ __forceinline__ void publish(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t look(const uint64_t* p) { return __hip_atomic_load(const_cast<uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// the ticket of the workgroup
+__device__ __forceinline__ unsigned draw(const GlrP& p, unsigned* place) {
+  if (threadIdx.x == 0) *place = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return (unsigned)__builtin_amdgcn_readfirstlane((int)*place);
+}
+// Waits for a word.  (Its workgroup has a lower ticket: it runs, and waits for lower ones only.)
+__device__ __forceinline__ uint64_t await(const uint64_t* p) {
+  uint64_t v;
+  while ((v = look(p)) == NOTHING) __builtin_amdgcn_s_sleep(1);
+  return v;
+}
+// What a chained workgroup keeps in LDS: the maps of its waves, those of the tiles before it in its group, the state before the group, the ticket.
+template <int VEC>
+struct ChainLds {
+  float2* waves;                 // [nw][VEC][64]
+  float2* tiles;                 // [GROUP - 1][VEC][64]
+  float* first;                  // [VEC][64]
+  unsigned* ticket;
+  __device__ explicit ChainLds(float2* lds) {
+    waves = lds;
+    tiles = waves + (blockDim.x >> 6) * VEC * 64;
+    first = reinterpret_cast<float*>(tiles + (GROUP - 1) * VEC * 64);
+    ticket = reinterpret_cast<unsigned*>(first + VEC * 64);
+  }
+  static size_t bytes(int nw) { return (size_t)(nw + GROUP - 1) * VEC * 64 * sizeof(float2) + VEC * 64 * sizeof(float) + 16; }
+};
+// tile_scan over workgroups: wave 0 publishes the tile's map, and every wave fetches its share of the words that the state before the tile is made of.
+template <int VEC, bool CUT, bool REV>
+__device__ __forceinline__ void chain_scan(const GlrP& p, const ChainLds<VEC>& lds, const Place<VEC>& at, const float (&A)[VEC], const float (&S)[VEC], float (&carry)[VEC],
+                                           float (&h)[VEC]) {
+  const int lane = threadIdx.x & 63, place = at.tile % GROUP, group = at.tile / GROUP;
+  const int64_t plane = p.a.B * p.a.D, row = at.b * p.a.D + at.ch0;
+  float tA[VEC], tS[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; i++) tA[i] = 1.f, tS[i] = 0.f;
+  put_map<VEC>(lds.waves, at, A, S);
+  __syncthreads();
+  if (at.w == 0 && at.tile + 1 < p.ntile) {
+    float none[VEC];
+    fold_waves<VEC, CUT, REV>(lds.waves, at, tS, none);
+    for (int q = 0; q < at.nw; q++)
+#pragma unroll
+      for (int i = 0; i < VEC; i++) tA[i] = map_a<CUT>(tA[i], lds.waves[(q * VEC + i) * 64 + lane].x);
+    if (at.chan && place + 1 < GROUP)
+#pragma unroll
+      for (int i = 0; i < VEC; i++) publish(p.map + (int64_t)at.tile * plane + row + at.off + i, word(tS[i], tA[i]));
+  }
+  for (int q = at.w; q < place; q += at.nw)
+#pragma unroll
+    for (int i = 0; i < VEC; i++) {
+      const uint64_t v = await(p.map + (int64_t)(group * GROUP + q) * plane + row + at.off + i);
+      lds.tiles[(q * VEC + i) * 64 + lane] = make_float2(high(v), low(v));
+    }
+  if (at.w == at.nw - 1) {
+    float f[VEC];
+    if (group == 0) get_state<VEC>(p.state0, row, at, f);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) lds.first[i * 64 + lane] = group == 0 ? f[i] : low(await(p.behind + (int64_t)(group - 1) * plane + row + at.off + i));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < VEC; i++) carry[i] = lds.first[i * 64 + lane];
+  for (int q0 = 0; q0 < place; q0 += 4) {
+    float2 m[4][VEC];
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+      for (int i = 0; i < VEC; i++) m[k][i] = lds.tiles[((q0 + k < place ? q0 + k : q0) * VEC + i) * 64 + lane];
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (q0 + k < place)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) carry[i] = map_s<CUT>(m[k][i].x, carry[i], m[k][i].y);
+  }
+  if (at.w == 0 && at.chan && place + 1 == GROUP && at.tile + 1 < p.ntile)
+#pragma unroll
+    for (int i = 0; i < VEC; i++) publish(p.behind + (int64_t)group * plane + row + at.off + i, word(map_s<CUT>(tA[i], carry[i], tS[i]), 0.f));
+  fold_waves<VEC, CUT, REV>(lds.waves, at, carry, h);
+}
+// clears what a chain's words start from
+__global__ __launch_bounds__(256) void k_chain_init(GlrP p, const float* first, int64_t words) {
+  const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x, n = p.a.B * p.a.D;
+  if (i0 == 0) *p.ticket = 0;
+  for (int64_t i = i0; i < words; i += (int64_t)gridDim.x * 256) p.map[i] = NOTHING;
+  for (int64_t i = i0; i < n; i += (int64_t)gridDim.x * 256) p.state0[i] = first ? first[i] : 0.f;
+}
+
+// ---- forward: a workgroup takes 64 VEC channels of one sequence through time, nw segments (a tile) at a time; CHAIN: one tile ---------------------------
+template <int DT, int VEC, bool TANH, bool CUT, bool CHAIN>
+__global__ __launch_bounds__(64 * MAXW / VEC) void k_glr(GlrP p) {
+  extern __shared__ float2 lds[];          // 2 x [nw][VEC][64]; CHAIN: ChainLds
+  const hiertcn_glr_t& a = p.a;
+  const ChainLds<VEC> chain(lds);
+  const Place<VEC> at(p, CHAIN ? draw(p, chain.ticket) : blockIdx.x);
+  const int64_t row = at.b * a.D + at.ch0;
+  const int len = length_of(a, at.b), seg0 = CHAIN ? at.tile * at.nw : 0, seg1 = CHAIN && seg0 + at.nw < p.nseg ? seg0 + at.nw : p.nseg;
+  float carry[VEC], h[VEC], u[SEG][VEC], s[SEG][VEC], A[VEC], S[VEC];
+  typename OpsRaw<DT, VEC>::type rg[SEG], rc[SEG];
+  if (!CHAIN) get_state<VEC>(a.state_in, row, at, carry);
+  int turn = 0;
+  for (int g0 = seg0; g0 < seg1; g0 += at.nw, turn ^= 1) {
+    const int g = g0 + at.w, t0 = g * SEG, n = clamped(len - t0, 0, SEG), nrow = g < seg1 ? clamped((int)a.T - t0, 0, SEG) : 0;
+    uint32_t keep = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < VEC; i++) A[i] = 1.f, S[i] = 0.f;
+    if (n > 0) {
+      const float mask = load_mask<CUT>(a, at.b, t0, n);
+      load_rows<DT, VEC>(a.gate, at.b * a.gate_sb + t0 * a.gate_st + at.ch0, a.gate_st, at.off, n, rg);
+      load_rows<DT, VEC>(a.cand, at.b * a.cand_sb + t0 * a.cand_st + at.ch0, a.cand_st, at.off, n, rc);
+      __builtin_amdgcn_sched_barrier(0);
+      keep = __builtin_amdgcn_readfirstlane(keep_bits<CUT>(mask, n));
+#pragma unroll
+      for (int j = 0; j < SEG; j++) {
+        float g4[VEC], c4[VEC];
+        ops_cvt<DT, VEC>(rg[j], g4);
+        ops_cvt<DT, VEC>(rc[j], c4);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          float w;
+          gate_of(g4[i], u[j][i], w);
+          s[j][i] = w * (TANH ? tanh_of(c4[i]) : c4[i]);
+        }
+      }
+      if (n < SEG)                         // dead steps: the identity
+#pragma unroll
+        for (int j = 1; j < SEG; j++)
+#pragma unroll
+          for (int i = 0; i < VEC; i++)
+            if (j >= n) u[j][i] = 1.f, s[j][i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < SEG; j++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          S[i] = fmaf(u[j][i], held<CUT>(S[i], keep, j), s[j][i]);
+          A[i] *= u[j][i];
+        }
+      close_map<VEC, CUT>(keep, A);
+    }
+    if (CHAIN) chain_scan<VEC, CUT, false>(p, chain, at, A, S, carry, h);
+    else tile_scan<VEC, CUT, false>(lds + turn * at.nw * VEC * 64, at, A, S, carry, h);
+    if (a.record && nrow > 0) put_state<VEC>(a.record, (at.b * p.nseg + g) * a.D + at.ch0, at, h);
+    if (CUT) keep = anew(keep);
+    const char* o = row_ptr<DT>(a.out, at.b * a.out_sb + t0 * a.out_st + at.ch0);
+    if (n > 0)
+#pragma unroll
+      for (int j = 0; j < SEG; j++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          h[i] = fmaf(u[j][i], held<CUT>(h[i], keep, j), s[j][i]);
+          s[j][i] = j < n ? h[i] : 0.f;
+        }
+    else
+#pragma unroll
+      for (int j = 0; j < SEG; j++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) s[j][i] = 0.f;
+    store_rows<DT, VEC>(o, a.out_st, at, nrow, s);
+  }
+  if (at.w == 0 && a.state_out && seg1 == p.nseg) put_state<VEC>(a.state_out, row, at, carry);
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------------------------------
-// Per element of a segment: u, fg = (h_prev - c) u (1 - u) and fx = (1 - u) act'(c), so that dgate = lambda fg and dcand = lambda fx; d = dout.
-// h: the state before the segment (the record).
-template <int DT, int VEC, bool TANH>
-__device__ __forceinline__ void load_backward(const hiertcn_glr_t& a, int64_t b, int64_t t0, int64_t ch, int n, uint32_t keep, float (&h)[VEC], float (&u)[SEG][VEC],
-                                              float (&fg)[SEG][VEC], float (&fx)[SEG][VEC], float (&d)[SEG][VEC]) {
-  if (n > 0) {
-    load_rows<DT, VEC>(a.gate, b * a.gate_sb + t0 * a.gate_st + ch, a.gate_st, n, u);
-    load_rows<DT, VEC>(a.cand, b * a.cand_sb + t0 * a.cand_st + ch, a.cand_st, n, fx);
-    load_rows<DT, VEC>(a.dout, b * a.dout_sb + t0 * a.dout_st + ch, a.dout_st, n, d);
-  }
-#pragma unroll
-  for (int j = 0; j < SEG; j++)
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      if (j < n) {
-        float w;
-        gate_of(u[j][i], u[j][i], w);
-        const float c = TANH ? tanh_of(fx[j][i]) : fx[j][i];
-        const float hp = keep >> j & 1 ? h[i] : 0.f;
-        h[i] = fmaf(u[j][i], hp, w * c);
-        fg[j][i] = (hp - c) * (u[j][i] * w);
-        fx[j][i] = TANH ? w * fmaf(-c, c, 1.f) : w;
-      } else {
-        u[j][i] = 1.f;
-        fg[j][i] = fx[j][i] = d[j][i] = 0.f;
-      }
-    }
-}
-// r -> A r + Q of a segment, last step first
-template <int VEC>
-__device__ __forceinline__ void segment_map_rev(const float (&u)[SEG][VEC], const float (&d)[SEG][VEC], uint32_t keep, float (&A)[VEC], float (&Q)[VEC]) {
-#pragma unroll
-  for (int i = 0; i < VEC; i++) A[i] = 1.f, Q[i] = 0.f;
-#pragma unroll
-  for (int j = SEG - 1; j >= 0; j--)
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      Q[i] = keep >> j & 1 ? u[j][i] * (d[j][i] + Q[i]) : 0.f;
-      A[i] *= u[j][i];
-    }
-#pragma unroll
-  for (int i = 0; i < VEC; i++) A[i] = keep == 0xffffffffu ? (A[i] == A[i] ? fmaxf(A[i], TINY) : A[i]) : 0.f;
-}
-// gradients of a segment, given r behind it; r before it afterwards
-template <int DT, int VEC>
-__device__ __forceinline__ void replay_rev(const hiertcn_glr_t& a, int64_t b, int64_t t0, int64_t ch, bool chan, int n, int nrow, uint32_t keep, const float (&u)[SEG][VEC],
-                                           const float (&fg)[SEG][VEC], const float (&fx)[SEG][VEC], const float (&d)[SEG][VEC], float (&r)[VEC]) {
-  const int64_t bg = b * a.dgate_sb + t0 * a.dgate_st + ch, bc = b * a.dcand_sb + t0 * a.dcand_st + ch;
-#pragma unroll
-  for (int j = SEG - 1; j >= 0; j--) {
-    float og[VEC], oc[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      const float lam = d[j][i] + r[i];
-      og[i] = j < n ? lam * fg[j][i] : 0.f;
-      oc[i] = j < n ? lam * fx[j][i] : 0.f;
-      r[i] = keep >> j & 1 ? u[j][i] * lam : 0.f;      // (a step behind the end has u = 1, d = 0: r passes)
-    }
-    if (j < nrow && chan) {
-      ops_st<DT, VEC>(a.dgate, bg + j * a.dgate_st, og);
-      ops_st<DT, VEC>(a.dcand, bc + j * a.dcand_st, oc);
-    }
-  }
-}
-
-template <int DT, int VEC, bool TANH>
-__global__ __launch_bounds__(64) void k_glr_seq_bwd(GlrP p) {
+// Per element: u, fg = (h_prev - c) u (1 - u) and fx = (1 - u) act'(c), so that dgate = lambda fg and dcand = lambda fx; d = dout.
+// CHAIN: the tiles in the order of the tickets are the sequence's from its end.
+template <int DT, int VEC, bool TANH, bool CUT, bool CHAIN>
+__global__ __launch_bounds__(64 * MAXW) void k_glr_bwd(GlrP p) {
+  extern __shared__ float2 lds[];          // as in k_glr
   const hiertcn_glr_t& a = p.a;
-  const int64_t groups = a.D / VEC, id = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (id >= a.B * groups) return;
-  const int64_t b = id / groups, ch = id % groups * VEC;
-  const int64_t len = length_of(a, b);
-  float r[VEC], h[VEC], u[SEG][VEC], fg[SEG][VEC], fx[SEG][VEC], d[SEG][VEC];
-  get_state<VEC>(a.dstate_out, b, a.D, ch, r);
-  for (int64_t g = p.nseg - 1; g >= 0; g--) {
-    const int64_t t0 = g * SEG;
-    const int n = (int)clamp64(len - t0, 0, SEG), nrow = (int)clamp64(a.T - t0, 0, SEG);
-    get_state<VEC>(a.record + g * a.D, b, p.nseg * a.D, ch, h);
-    const uint32_t keep = keep_bits(a, b, t0, n);
-    load_backward<DT, VEC, TANH>(a, b, t0, ch, n, keep, h, u, fg, fx, d);
-    replay_rev<DT, VEC>(a, b, t0, ch, true, n, nrow, keep, u, fg, fx, d, r);
-  }
-  if (a.dstate_in) ops_st<HIERTCN_FP32, VEC>(a.dstate_in, b * a.D + ch, r);
-}
-
-template <int DT, int VEC, bool TANH>
-__global__ __launch_bounds__(1024) void k_glr_tile_bwd(GlrP p) {
-  constexpr int CL = CB / VEC, TS = 64 / CL;
-  __shared__ float2 lds[2][16 * CB];
-  const hiertcn_glr_t& a = p.a;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, ts = lane / CL, cl = lane % CL;
-  const int64_t blk = blockIdx.x, cb = blk % p.ncb, b = blk / p.ncb % a.B, chunk = blk / p.ncb / a.B;
-  const bool chan = cb * CB + cl * VEC < a.D;
-  const int64_t ch = chan ? cb * CB + cl * VEC : 0;
-  const int64_t len = length_of(a, b);
-  const int tile_seg = nw * TS;
-  const int64_t seg0 = chunk * p.chunk_tiles * tile_seg;
-  const int64_t seg1 = chunk + 1 < p.nchunk ? seg0 + (int64_t)p.chunk_tiles * tile_seg : p.nseg;
-  const int64_t tiles = (seg1 - seg0 + tile_seg - 1) / tile_seg;
+  const ChainLds<VEC> chain(lds);
+  const Place<VEC> at(p, CHAIN ? draw(p, chain.ticket) : blockIdx.x);
+  const int64_t row = at.b * a.D + at.ch0;
+  const int len = length_of(a, at.b), seg0 = CHAIN ? (p.ntile - 1 - at.tile) * at.nw : 0, seg1 = CHAIN && seg0 + at.nw < p.nseg ? seg0 + at.nw : p.nseg;
+  const int tiles = (seg1 - seg0 + at.nw - 1) / at.nw;
   float carry[VEC], r[VEC], h[VEC], u[SEG][VEC], fg[SEG][VEC], fx[SEG][VEC], d[SEG][VEC], A[VEC], Q[VEC];
-  get_state<VEC>(a.dstate_out, b, a.D, ch, carry);
-  for (int64_t q = p.nchunk - 1; q > chunk; q--)
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      const float2 m = p.agg[(q * a.B + b) * a.D + ch + i];
-      carry[i] = map_s(m.x, carry[i], m.y);
-    }
+  typename OpsRaw<DT, VEC>::type rg[SEG], rc[SEG], rd[SEG];
+  if (!CHAIN) get_state<VEC>(a.dstate_out, row, at, carry);
   int turn = 0;
-  for (int64_t k = tiles - 1; k >= 0; k--, turn ^= 1) {
-    const int64_t g = seg0 + k * tile_seg + w * TS + ts, t0 = g * SEG;
-    const int nrow = g < seg1 ? (int)clamp64(a.T - t0, 0, SEG) : 0, n = g < seg1 ? (int)clamp64(len - t0, 0, SEG) : 0;
-    get_state<VEC>(n > 0 ? a.record + g * a.D : nullptr, b, p.nseg * a.D, ch, h);
-    const uint32_t keep = keep_bits(a, b, t0, n);
-    load_backward<DT, VEC, TANH>(a, b, t0, ch, n, keep, h, u, fg, fx, d);
-    segment_map_rev<VEC>(u, d, keep, A, Q);
-    tile_scan<VEC, true>(lds[turn], nw, w, ts, cl, A, Q, carry, r);
-    replay_rev<DT, VEC>(a, b, t0, ch, chan, n, nrow, keep, u, fg, fx, d, r);
-  }
-  if (w == 0 && ts == 0 && chan && a.dstate_in && chunk == 0) ops_st<HIERTCN_FP32, VEC>(a.dstate_in, b * a.D + ch, carry);
-}
-
-// the chunks' maps of the backward recurrence (gates and dout only)
-template <int DT, int VEC>
-__global__ __launch_bounds__(1024) void k_glr_agg_bwd(GlrP p) {
-  constexpr int CL = CB / VEC, TS = 64 / CL;
-  __shared__ float2 lds[2][16 * CB];
-  const hiertcn_glr_t& a = p.a;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, ts = lane / CL, cl = lane % CL;
-  const int64_t blk = blockIdx.x, cb = blk % p.ncb, b = blk / p.ncb % a.B, chunk = blk / p.ncb / a.B;
-  const bool chan = cb * CB + cl * VEC < a.D;
-  const int64_t ch = chan ? cb * CB + cl * VEC : 0;
-  const int64_t len = length_of(a, b);
-  const int tile_seg = nw * TS;
-  const int64_t seg0 = chunk * p.chunk_tiles * tile_seg;
-  const int64_t seg1 = chunk + 1 < p.nchunk ? seg0 + (int64_t)p.chunk_tiles * tile_seg : p.nseg;
-  const int64_t live = seg1 * SEG < len ? seg1 : (len + SEG - 1) / SEG;      // segments behind the end are identities
-  const int64_t tiles = live > seg0 ? (live - seg0 + tile_seg - 1) / tile_seg : 0;
-  float carry[VEC], carryA[VEC], none[VEC], u[SEG][VEC], d[SEG][VEC], A[VEC], Q[VEC];
+  for (int k = tiles - 1; k >= 0; k--, turn ^= 1) {
+    const int g = seg0 + k * at.nw + at.w, t0 = g * SEG;
+    const int nrow = g < seg1 ? clamped((int)a.T - t0, 0, SEG) : 0, n = g < seg1 ? clamped(len - t0, 0, SEG) : 0;
+    uint32_t keep = 0xffffffffu;
 #pragma unroll
-  for (int i = 0; i < VEC; i++) carry[i] = 0.f, carryA[i] = 1.f;
-  int turn = 0;
-  for (int64_t k = tiles - 1; k >= 0; k--, turn ^= 1) {
-    const int64_t g = seg0 + k * tile_seg + w * TS + ts, t0 = g * SEG;
-    const int n = g < seg1 ? (int)clamp64(len - t0, 0, SEG) : 0;
+    for (int i = 0; i < VEC; i++) A[i] = 1.f, Q[i] = 0.f;
     if (n > 0) {
-      load_rows<DT, VEC>(a.gate, b * a.gate_sb + t0 * a.gate_st + ch, a.gate_st, n, u);
-      load_rows<DT, VEC>(a.dout, b * a.dout_sb + t0 * a.dout_st + ch, a.dout_st, n, d);
-    }
+      const float mask = load_mask<CUT>(a, at.b, t0, n);
+      get_state<VEC>(a.record, (at.b * p.nseg + g) * a.D + at.ch0, at, h);
+      load_rows<DT, VEC>(a.gate, at.b * a.gate_sb + t0 * a.gate_st + at.ch0, a.gate_st, at.off, n, rg);
+      load_rows<DT, VEC>(a.cand, at.b * a.cand_sb + t0 * a.cand_st + at.ch0, a.cand_st, at.off, n, rc);
+      load_rows<DT, VEC>(a.dout, at.b * a.dout_sb + t0 * a.dout_st + at.ch0, a.dout_st, at.off, n, rd);
+      __builtin_amdgcn_sched_barrier(0);
+      keep = __builtin_amdgcn_readfirstlane(keep_bits<CUT>(mask, n));
 #pragma unroll
-    for (int j = 0; j < SEG; j++)
+      for (int j = 0; j < SEG; j++) {
+        float g4[VEC], c4[VEC];
+        ops_cvt<DT, VEC>(rg[j], g4);
+        ops_cvt<DT, VEC>(rc[j], c4);
+        ops_cvt<DT, VEC>(rd[j], d[j]);
 #pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        float wv;
-        if (j < n) gate_of(u[j][i], u[j][i], wv);
-        else u[j][i] = 1.f, d[j][i] = 0.f;
+        for (int i = 0; i < VEC; i++) {
+          float w;
+          gate_of(g4[i], u[j][i], w);
+          const float c = TANH ? tanh_of(c4[i]) : c4[i];
+          const float hp = held<CUT>(h[i], keep, j);
+          h[i] = fmaf(u[j][i], hp, w * c);
+          fg[j][i] = (hp - c) * (u[j][i] * w);
+          fx[j][i] = TANH ? w * fmaf(-c, c, 1.f) : w;
+        }
       }
-    segment_map_rev<VEC>(u, d, keep_bits(a, b, t0, n), A, Q);
-    tile_scan<VEC, true>(lds[turn], nw, w, ts, cl, A, Q, carry, none);
-    for (int q = 0; q < nw; q++)
+      if (n < SEG)                         // dead steps: the identity, no gradient
 #pragma unroll
-      for (int i = 0; i < VEC; i++) carryA[i] = map_a(carryA[i], lds[turn][q * CB + cl * VEC + i].x);
+        for (int j = 1; j < SEG; j++)
+#pragma unroll
+          for (int i = 0; i < VEC; i++)
+            if (j >= n) u[j][i] = 1.f, fg[j][i] = fx[j][i] = d[j][i] = 0.f;
+#pragma unroll
+      for (int j = SEG - 1; j >= 0; j--)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          Q[i] = held<CUT>(u[j][i] * (d[j][i] + Q[i]), keep, j);
+          A[i] *= u[j][i];
+        }
+      close_map<VEC, CUT>(keep, A);
+    }
+    if (CHAIN) chain_scan<VEC, CUT, true>(p, chain, at, A, Q, carry, r);
+    else tile_scan<VEC, CUT, true>(lds + turn * at.nw * VEC * 64, at, A, Q, carry, r);
+    if (CUT) keep = anew(keep);
+    if (n > 0)
+#pragma unroll
+      for (int j = SEG - 1; j >= 0; j--)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          const float lam = d[j][i] + r[i];
+          fg[j][i] *= lam;                 // (a dead step has fg = fx = 0)
+          fx[j][i] *= lam;
+          r[i] = held<CUT>(u[j][i] * lam, keep, j);
+        }
+    else
+#pragma unroll
+      for (int j = 0; j < SEG; j++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) fg[j][i] = fx[j][i] = 0.f;
+    store_rows<DT, VEC>(row_ptr<DT>(a.dgate, at.b * a.dgate_sb + t0 * a.dgate_st + at.ch0), a.dgate_st, at, nrow, fg);
+    store_rows<DT, VEC>(row_ptr<DT>(a.dcand, at.b * a.dcand_sb + t0 * a.dcand_st + at.ch0), a.dcand_st, at, nrow, fx);
   }
-  if (w == 0 && ts == 0 && chan)
-#pragma unroll
-    for (int i = 0; i < VEC; i++) p.agg[(chunk * a.B + b) * a.D + ch + i] = make_float2(carryA[i], carry[i]);
+  if (at.w == 0 && a.dstate_in && seg0 == 0) put_state<VEC>(a.dstate_in, row, at, carry);
 }
 
 // ---- launch selection --------------------------------------------------------------------------------------------------------------------------------
-struct Plan { bool seq; int nw, nchunk, chunk_tiles; int64_t ncb; };
+struct Plan { int vec, nw; bool chain; int64_t ncb, ntile; };
 
-// vec: channels of a thread (1 where the width, a stride or an address is odd)
-Plan plan_of(int64_t B, int64_t T, int64_t D, int vec, int most_waves) {
+// wide: the width, every stride and every address allow two channels of a thread at a time.  Measured on (lanes x steps x width), us, forward / backward:
+//   two channels where that still leaves 8 waves a SIMD: 512 x 500 x 256 bf16 95 against 119; else one, for the waves: 64 x 500 x 256 18.5 against 31
+//   one workgroup through a sequence where there are 256 of them: 64 x 500 x 256 19 / 28 against 25 / 35 chained; chained where there are fewer:
+//   2 x 65536 x 512 116 / 190 against 1670 / 2210, 8 x 500 x 256 12 / 14 against 16 / 23
+//   waves of a workgroup: as few as make 4096 in all (4096 x 30 x 256 one: 49 / 76, two 65 / 130 before; 512 x 500 x 256 four: 95 / 153, eight 97 / 160); chained
+//   eight (2 x 65536 x 512 132 / 189 against 160 / 215 with sixteen), but sixteen where those are one generation of workgroups (17 x 1001 x 333 24 against 27)
+Plan plan_of(int64_t B, int64_t T, int64_t D, bool wide, bool backward) {
   Plan q{};
-  const int ts = vec;                          // segments of a wave: 64 lanes / (64 channels / vec)
   const int64_t nseg = (T + SEG - 1) / SEG;
-  q.ncb = (D + CB - 1) / CB;
-  const int64_t seq_waves = (B * ((D + vec - 1) / vec) + 63) / 64;
-  q.seq = nseg <= 1 || seq_waves >= 4096;
-  q.nw = (int)((nseg + ts - 1) / ts < most_waves ? (nseg + ts - 1) / ts : most_waves);
-  if (q.nw < 1) q.nw = 1;
-  const int64_t tiles = (nseg + (int64_t)q.nw * ts - 1) / ((int64_t)q.nw * ts), wgs = B * q.ncb;
-  int64_t want = wgs >= 512 ? 1 : (1024 + wgs - 1) / wgs;
-  if (want > 64) want = 64;
-  if (want > tiles) want = tiles;
-  if (want < 1) want = 1;
-  q.chunk_tiles = (int)((tiles + want - 1) / want);
-  q.nchunk = (int)((tiles + q.chunk_tiles - 1) / q.chunk_tiles);
-  if (q.nchunk < 1) q.nchunk = 1;
+  q.vec = wide && !backward && B * ((D + 127) / 128) * nseg >= 8192 ? 2 : 1;
+  q.ncb = (D + 64 * q.vec - 1) / (64 * q.vec);
+  const int64_t wgs = B * q.ncb, generation = wgs * ((nseg + MAXW - 1) / MAXW);
+  q.chain = nseg > MAXW && wgs < 256;
+  const int64_t waves = !q.chain ? (4096 + wgs - 1) / wgs : generation >= 256 && generation <= 512 ? MAXW : 8;
+  const int most = MAXW / q.vec;               // (what the registers of a workgroup allow)
+  q.nw = (int)(waves > most ? most : waves < 1 ? 1 : waves);
+  if (q.nw > nseg) q.nw = (int)nseg;
+  q.ntile = (nseg + q.nw - 1) / q.nw;
   return q;
 }
-constexpr int FWD_WAVES = 16, BWD_WAVES = 16;
+int64_t words_of(const Plan& q, int64_t B, int64_t D) { return (q.ntile + q.ntile / GROUP + 1) * B * D; }
+size_t bytes_of(const Plan& q, int64_t B, int64_t D) { return q.chain ? (size_t)words_of(q, B, D) * 8 + (size_t)(B * D) * 4 + 16 : 0; }
 
 size_t workspace_of(int64_t B, int64_t T, int64_t D) {
   size_t most = 0;
-  for (int vec = 1; vec <= 2; vec++)
-    for (int waves : {FWD_WAVES, BWD_WAVES}) {
-      const Plan q = plan_of(B, T, D, vec, waves);
-      const size_t need = q.seq || q.nchunk == 1 ? 0 : (size_t)(q.nchunk * B * D) * sizeof(float2) + (size_t)(B * D) * sizeof(float);
+  for (bool wide : {false, true})
+    for (bool backward : {false, true}) {
+      const size_t need = bytes_of(plan_of(B, T, D, wide, backward), B, D);
       if (need > most) most = need;
     }
   return most;
@@ -485,8 +503,8 @@ size_t workspace_of(int64_t B, int64_t T, int64_t D) {
 int check_shape(const hiertcn_glr_t* a) {
   if (!a) return ops_fail(HIERTCN_ERR_INVALID, "null argument");
   if (a->B < 0 || a->T < 0 || a->D < 0) return ops_fail(HIERTCN_ERR_INVALID, "negative size");
-  if (a->B > (1ll << 31) || a->T > (1ll << 31) || a->D > (1ll << 31) || (a->B && a->D && a->B * a->D > (1ll << 40)))
-    return ops_fail(HIERTCN_ERR_INVALID, "B, T, D are at most 2^31, B * D at most 2^40");
+  if (a->B > (1ll << 31) || a->T >= (1ll << 31) - 1024 || a->D > (1ll << 31) || (a->B && a->D && a->B * a->D > (1ll << 40)))
+    return ops_fail(HIERTCN_ERR_INVALID, "B and D are at most 2^31, T below 2^31 - 1024, B * D at most 2^40");
   if (!ops_dtype_ok(a->dtype)) return ops_fail(HIERTCN_ERR_INVALID, "dtype %d: 0 fp32, 1 bf16, 2 fp16", a->dtype);
   if (a->cand_act != 0 && a->cand_act != 1) return ops_fail(HIERTCN_ERR_INVALID, "cand_act %d: 0 none, 1 tanh", a->cand_act);
   return HIERTCN_OK;
@@ -495,51 +513,33 @@ int check_shape(const hiertcn_glr_t* a) {
 // all addresses and strides of an operand allow `vec` elements at a time
 bool aligned(const void* p, int64_t sb, int64_t st, int es, int vec) { return !p || ((uintptr_t)p % (size_t)(es * vec) == 0 && sb % vec == 0 && st % vec == 0); }
 
-template <int DT, int VEC, bool TANH>
-hipError_t go_forward(GlrP& p, const Plan& q, hipStream_t st) {
-  const hiertcn_glr_t& a = p.a;
-  if (q.seq) {
-    const int64_t threads = a.B * (a.D / VEC);
-    hipLaunchKernelGGL((k_glr_seq<DT, VEC, TANH>), dim3((unsigned)((threads + 63) / 64)), dim3(64), 0, st, p);
+template <int DT, int VEC, bool TANH, bool CUT>
+hipError_t go(const GlrP& p, const Plan& q, bool backward, hipStream_t st) {
+  const dim3 grid((unsigned)(q.ncb * p.a.B * (q.chain ? q.ntile : 1))), block(64 * q.nw);
+  const size_t maps = (size_t)q.nw * q.vec * 64 * sizeof(float2);
+  if (q.chain) {
+    const int64_t words = words_of(q, p.a.B, p.a.D);
+    hipLaunchKernelGGL(k_chain_init, dim3((unsigned)(words / 1024 + 1 < 2048 ? words / 1024 + 1 : 2048)), dim3(256), 0, st, p, backward ? p.a.dstate_out : p.a.state_in, words);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const size_t lds = q.vec == 2 ? ChainLds<2>::bytes(q.nw) : ChainLds<1>::bytes(q.nw);
+    if (backward) hipLaunchKernelGGL((k_glr_bwd<DT, 1, TANH, CUT, true>), grid, block, lds, st, p);
+    else hipLaunchKernelGGL((k_glr<DT, VEC, TANH, CUT, true>), grid, block, lds, st, p);
     return hipGetLastError();
   }
-  const dim3 grid((unsigned)(q.ncb * a.B * q.nchunk)), block(64 * q.nw);
-  if (q.nchunk > 1) {
-    hipLaunchKernelGGL((k_glr_tile<DT, VEC, TANH, true>), grid, block, 0, st, p);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  hipLaunchKernelGGL((k_glr_tile<DT, VEC, TANH, false>), grid, block, 0, st, p);
+  const size_t lds = q.nw > 1 ? 2 * maps : 0;
+  if (backward) hipLaunchKernelGGL((k_glr_bwd<DT, 1, TANH, CUT, false>), grid, block, lds, st, p);
+  else hipLaunchKernelGGL((k_glr<DT, VEC, TANH, CUT, false>), grid, block, lds, st, p);
   return hipGetLastError();
 }
-template <int DT, int VEC, bool TANH>
-hipError_t go_backward(GlrP& p, const Plan& q, hipStream_t st) {
-  const hiertcn_glr_t& a = p.a;
-  if (q.seq) {
-    const int64_t threads = a.B * (a.D / VEC);
-    hipLaunchKernelGGL((k_glr_seq_bwd<DT, VEC, TANH>), dim3((unsigned)((threads + 63) / 64)), dim3(64), 0, st, p);
-    return hipGetLastError();
-  }
-  const dim3 grid((unsigned)(q.ncb * a.B * q.nchunk)), block(64 * q.nw);
-  if (q.nchunk > 1) {
-    hipLaunchKernelGGL((k_glr_agg_bwd<DT, VEC>), grid, block, 0, st, p);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  hipLaunchKernelGGL((k_glr_tile_bwd<DT, VEC, TANH>), grid, block, 0, st, p);
-  return hipGetLastError();
+template <int DT, int VEC>
+hipError_t go_act(const GlrP& p, const Plan& q, bool backward, hipStream_t st) {
+  if (p.a.cand_act) return p.a.mask ? go<DT, VEC, true, true>(p, q, backward, st) : go<DT, VEC, true, false>(p, q, backward, st);
+  return p.a.mask ? go<DT, VEC, false, true>(p, q, backward, st) : go<DT, VEC, false, false>(p, q, backward, st);
 }
-template <int VEC>
-hipError_t go(GlrP& p, const Plan& q, bool backward, hipStream_t st) {
-#define GLR_GO(DT)                                                                                                                   \
-  return backward ? (p.a.cand_act ? go_backward<DT, VEC, true>(p, q, st) : go_backward<DT, VEC, false>(p, q, st))                     \
-                  : (p.a.cand_act ? go_forward<DT, VEC, true>(p, q, st) : go_forward<DT, VEC, false>(p, q, st))
-  switch (p.a.dtype) {
-    case HIERTCN_FP32: GLR_GO(HIERTCN_FP32);
-    case HIERTCN_BF16: GLR_GO(HIERTCN_BF16);
-    default: GLR_GO(HIERTCN_FP16);
-  }
-#undef GLR_GO
+template <int DT>
+hipError_t go_vec(const GlrP& p, const Plan& q, bool backward, hipStream_t st) {
+  return q.vec == 2 ? go_act<DT, 2>(p, q, backward, st) : go_act<DT, 1>(p, q, backward, st);
 }
 
 int glr(const hiertcn_glr_t* in, bool backward, hipStream_t st) {
@@ -598,27 +598,26 @@ int glr(const hiertcn_glr_t* in, bool backward, hipStream_t st) {
     if ((uintptr_t)q % 4) return ops_fail(HIERTCN_ERR_INVALID, "an fp32 / int32 pointer is not a multiple of 4");
   for (const void* q : {a.gate, a.cand, (const void*)a.out, a.dout, (const void*)a.dgate, (const void*)a.dcand})
     if ((uintptr_t)q % (size_t)es) return ops_fail(HIERTCN_ERR_INVALID, "a pointer is not a multiple of its element");
-  int vec = a.D % 2 == 0 ? 2 : 1;
+  bool wide = a.D % 2 == 0;
   for (const void* q : f32)
-    if ((uintptr_t)q % 8 && q != a.mask && q != a.lengths) vec = 1;
-  if (!aligned(a.gate, a.gate_sb, a.gate_st, es, vec) || !aligned(a.cand, a.cand_sb, a.cand_st, es, vec) || !aligned(a.out, a.out_sb, a.out_st, es, vec) ||
-      !aligned(a.dout, a.dout_sb, a.dout_st, es, vec) || !aligned(a.dgate, a.dgate_sb, a.dgate_st, es, vec) || !aligned(a.dcand, a.dcand_sb, a.dcand_st, es, vec))
-    vec = 1;
-  const Plan q = plan_of(a.B, a.T, a.D, vec, backward ? BWD_WAVES : FWD_WAVES);
-  p.nseg = nseg;
+    if (q != a.mask && q != a.lengths && (uintptr_t)q % 8) wide = false;
+  wide = wide && aligned(a.gate, a.gate_sb, a.gate_st, es, 2) && aligned(a.cand, a.cand_sb, a.cand_st, es, 2) && aligned(a.out, a.out_sb, a.out_st, es, 2) &&
+         aligned(a.dout, a.dout_sb, a.dout_st, es, 2) && aligned(a.dgate, a.dgate_sb, a.dgate_st, es, 2) && aligned(a.dcand, a.dcand_sb, a.dcand_st, es, 2);
+  const Plan q = plan_of(a.B, a.T, a.D, wide, backward);
+  p.nseg = (int)nseg;
   p.ncb = (int)q.ncb;
-  p.nchunk = q.nchunk;
-  p.chunk_tiles = q.chunk_tiles;
-  if (!q.seq && q.nchunk > 1) {
+  p.ntile = (int)q.ntile;
+  if (q.ncb * a.B * (q.chain ? q.ntile : 1) > 0x7fffffffll) return ops_fail(HIERTCN_ERR_INVALID, "B * D is too large for one launch");
+  if (q.chain) {
     const size_t need = workspace_of(a.B, a.T, a.D);      // (the most that any alignment and direction takes)
     if (!a.workspace || a.workspace_bytes < need || (uintptr_t)a.workspace % 16)
       return ops_fail(HIERTCN_ERR_WORKSPACE, "workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", need, a.workspace ? a.workspace_bytes : (size_t)0);
-    p.agg = static_cast<float2*>(a.workspace);
-    p.state0 = reinterpret_cast<float*>(p.agg + q.nchunk * a.B * a.D);
+    p.map = static_cast<uint64_t*>(a.workspace);
+    p.behind = p.map + q.ntile * a.B * a.D;
+    p.state0 = reinterpret_cast<float*>(p.map + words_of(q, a.B, a.D));
+    p.ticket = reinterpret_cast<unsigned*>(p.state0 + a.B * a.D);
   }
-  const int64_t blocks = q.seq ? (a.B * ((a.D + vec - 1) / vec) + 63) / 64 : q.ncb * a.B * q.nchunk;
-  if (blocks > 0x7fffffffll) return ops_fail(HIERTCN_ERR_INVALID, "B * D is too large for one launch");
-  OPS_TRY(vec == 2 ? go<2>(p, q, backward, st) : go<1>(p, q, backward, st));
+  OPS_TRY(a.dtype == HIERTCN_FP32 ? go_vec<HIERTCN_FP32>(p, q, backward, st) : a.dtype == HIERTCN_BF16 ? go_vec<HIERTCN_BF16>(p, q, backward, st) : go_vec<HIERTCN_FP16>(p, q, backward, st));
   return HIERTCN_OK;
 }
 

@@ -84,5 +84,18 @@ __device__ __forceinline__ void ops_st(void* __restrict__ p, int64_t off, const 
     *reinterpret_cast<OpsH<VEC>*>(static_cast<uint16_t*>(p) + off) = x;
   }
 }
+// the same in two steps, so that many loads can be in flight before the first is converted
+template <int DT, int VEC>
+struct OpsRaw { typedef OpsH<VEC> type; };
+template <int VEC>
+struct OpsRaw<HIERTCN_FP32, VEC> { typedef OpsF<VEC> type; };
+template <int DT, int VEC>
+__device__ __forceinline__ void ops_cvt(const typename OpsRaw<DT, VEC>::type& x, float (&o)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; i++) {
+    if constexpr (DT == HIERTCN_FP32) o[i] = x.v[i];
+    else o[i] = ops_h2f(x.v[i], DT);
+  }
+}
 // 2^x through v_exp_f32 (one ulp); e^x for |x| that matter here
 __device__ __forceinline__ float ops_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }

@@ -23,9 +23,10 @@ _ACT = {"none": 0, "tanh": 1}
 def _rows(t, name, dtype, device, shape):
     """[B, T, D] with a contiguous last dimension and any other strides -> (pointer, stride of b, stride of t)."""
     need(t, name, dtype, device, shape, contiguous=False)
-    if t.shape[2] > 1 and t.stride(2) != 1:
-        raise HierTCNError(f"{name}: the last dimension must be contiguous (stride {t.stride(2)})")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    sb, st, sd = t.stride()
+    if sd != 1 and shape[2] > 1:
+        raise HierTCNError(f"{name}: the last dimension must be contiguous (stride {sd})")
+    return t.data_ptr(), sb, st
 
 
 def _common(gate, cand, mask, lengths, cand_act):
@@ -45,9 +46,11 @@ def _common(gate, cand, mask, lengths, cand_act):
         a.mask, a.mask_sb, a.mask_st = mask.data_ptr(), mask.stride(0), mask.stride(1)
     if lengths is not None:
         a.lengths = need(lengths, "lengths", torch.int32, device, shape[:1]).data_ptr()
-    ws = _ops.workspace(_ops.lib().hiertcn_glr_workspace_bytes(a.B, a.T, a.D), device)
-    if ws is not None:
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    ws = None
+    nbytes = _ops.size("hiertcn_glr_workspace_bytes", *shape)
+    if nbytes:
+        ws = _ops.workspace(nbytes, device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
     return a, device, ws
 
 
@@ -70,10 +73,10 @@ def glr_scan(gate: torch.Tensor, cand: torch.Tensor, state: Optional[torch.Tenso
         state_out.zero_()
         return h, state_out, torch.empty(0, dtype=torch.float32, device=device) if want_record else None
     a.state_out = state_out.data_ptr()
-    a.out, a.out_sb, a.out_st = h.data_ptr(), h.stride(0), h.stride(1)
+    a.out, a.out_sb, a.out_st = h.data_ptr(), T * D, D
     record = None
     if want_record:
-        record = torch.empty(_ops.lib().hiertcn_glr_record_floats(B, T, D), dtype=torch.float32, device=device)
+        record = torch.empty(_ops.size("hiertcn_glr_record_floats", B, T, D), dtype=torch.float32, device=device)
         a.record = record.data_ptr()
     _ops.call(_ops.lib().hiertcn_glr_forward, device, C.byref(a))
     return h, state_out, record
@@ -88,7 +91,7 @@ def glr_scan_backward(gate: torch.Tensor, cand: torch.Tensor, dh: torch.Tensor, 
     a, device, ws = _common(gate, cand, mask, lengths, cand_act)
     shape = gate.shape
     B, T, D = shape
-    need(record, "record", torch.float32, device, (_ops.lib().hiertcn_glr_record_floats(B, T, D),))
+    need(record, "record", torch.float32, device, (_ops.size("hiertcn_glr_record_floats", B, T, D),))
     a.record = record.data_ptr()
     a.dout, a.dout_sb, a.dout_st = _rows(dh, "dh", gate.dtype, device, shape)
     dgate = torch.empty(shape, dtype=gate.dtype, device=device) if dgate is None else dgate
@@ -111,9 +114,28 @@ def glr_step(gate: torch.Tensor, cand: torch.Tensor, state: torch.Tensor, mask: 
              cand_act: str = "tanh", state_out: Optional[torch.Tensor] = None):
     """One more step of every lane (serving): gate, cand [B, D], state [B, D] fp32, mask [B] fp32, active [B] int32 (0: the lane has no step -- its output is
     0 and its state stays) -> (h [B, D], state).  state_out: where the new state goes; `state` itself updates it in place."""
-    if not isinstance(gate, torch.Tensor) or not isinstance(cand, torch.Tensor):
-        raise TypeError("gate, cand: expected torch.Tensors")
-    if gate.dim() != 2 or cand.dim() != 2:
-        raise HierTCNError(f"gate, cand: shapes {tuple(gate.shape)}, {tuple(cand.shape)}, expected [B, D]")
-    h, state, _ = glr_scan(gate[:, None], cand[:, None], state, mask=None if mask is None else mask[:, None], lengths=active, cand_act=cand_act, state_out=state_out)
-    return h[:, 0], state
+    if isinstance(gate, torch.Tensor) and gate.dim() != 2:
+        raise HierTCNError(f"gate: shape {tuple(gate.shape)}, expected [B, D]")
+    device = _ops.on_gpu(gate, "gate")
+    if cand_act not in _ACT:
+        raise HierTCNError(f"cand_act {cand_act!r}: 'tanh' or 'none'")
+    shape = gate.shape
+    B, D = shape
+    need(cand, "cand", gate.dtype, device, shape, contiguous=False)
+    need(state, "state", torch.float32, device, shape)
+    (gb, gd), (cb, cd) = gate.stride(), cand.stride()
+    if D > 1 and (gd != 1 or cd != 1):
+        raise HierTCNError("gate, cand: the last dimension must be contiguous")
+    h = torch.empty(shape, dtype=gate.dtype, device=device)
+    if state_out is None:
+        state_out = torch.empty(shape, dtype=torch.float32, device=device)
+    elif state_out is not state:
+        need(state_out, "state_out", torch.float32, device, shape)
+    a = _ops.Glr(B, 1, D, _ops.DTYPE[gate.dtype], _ACT[cand_act], gate.data_ptr(), gb, 0, cand.data_ptr(), cb, 0)
+    if mask is not None:
+        a.mask, a.mask_sb = need(mask, "mask", torch.float32, device, (B,), contiguous=False).data_ptr(), mask.stride(0)
+    if active is not None:
+        a.lengths = need(active, "active", torch.int32, device, (B,)).data_ptr()
+    a.state_in, a.state_out, a.out, a.out_sb = state.data_ptr(), state_out.data_ptr(), h.data_ptr(), D
+    _ops.call(_ops.lib().hiertcn_glr_forward, device, C.byref(a))
+    return h, state_out

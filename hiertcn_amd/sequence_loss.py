@@ -22,10 +22,11 @@ _MEAN = {"sequence": 0, "token": 1}
 def _stride(t, name):
     """Row stride of [n, T, V] whose rows lie at one distance."""
     n, T, V = t.shape
-    if V > 1 and t.stride(2) != 1:
-        raise HierTCNError(f"{name}: the last dimension must be contiguous (stride {t.stride(2)})")
-    ld = t.stride(1) if T > 1 else t.stride(0) if n > 1 else V
-    if n > 1 and T > 1 and t.stride(0) != T * ld:
+    sn, st, sv = t.stride()
+    if V > 1 and sv != 1:
+        raise HierTCNError(f"{name}: the last dimension must be contiguous (stride {sv})")
+    ld = st if T > 1 else sn if n > 1 else V
+    if n > 1 and T > 1 and sn != T * ld:
         raise HierTCNError(f"{name}: rows must lie at one distance (strides {t.stride()})")
     return ld
 
@@ -48,9 +49,11 @@ def _rows(logits, ids, grad_scale=1.0, want_grad=False, dlogits=None):
         r.dlogits, r.dld = dlogits.data_ptr(), _stride(dlogits, "dlogits")
     elif dlogits is not None:
         raise HierTCNError("dlogits given, want_grad is False")
-    ws = _ops.workspace(_ops.lib().hiertcn_rows_workspace_bytes(n, T, V), device)
-    if ws is not None:
-        r.workspace, r.workspace_bytes = ws.data_ptr(), ws.numel()
+    ws = None
+    nbytes = _ops.size("hiertcn_rows_workspace_bytes", n, T, V)
+    if nbytes:
+        ws = _ops.workspace(nbytes, device)
+        r.workspace, r.workspace_bytes = ws.data_ptr(), nbytes
     return r, device, logp, dlogits, ws
 
 
@@ -74,11 +77,11 @@ def preference_loss(logits: torch.Tensor, ids: torch.Tensor, ref_logp: torch.Ten
     r, device, logp, dlogits, ws = _rows(logits, ids, grad_scale, want_grad, dlogits)
     P = r.n // 2
     need(ref_logp, "ref_logp", torch.float32, device, (r.n,))
-    buf = torch.empty(1 + 2 * P + r.n, dtype=torch.float32, device=device)
-    loss, pair, margin, seq = buf[0], buf[1:1 + P], buf[1 + P:1 + 2 * P], buf[1 + 2 * P:]
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    buf = torch.empty(4 * P, dtype=torch.float32, device=device)
+    pair, margin, seq = buf.split((P, P, 2 * P))
     base = buf.data_ptr()
-    q = _ops.Preference(kind=_KIND[kind], average=int(bool(average)), beta=beta, smoothing=label_smoothing, ref=ref_logp.data_ptr(), loss=base,
-                        pair_loss=base + 4, margin=base + 4 * (1 + P), seq_logp=base + 4 * (1 + 2 * P))
+    q = _ops.Preference(_KIND[kind], int(bool(average)), beta, label_smoothing, ref_logp.data_ptr(), loss.data_ptr(), base, base + 4 * P, base + 8 * P)
     _ops.call(_ops.lib().hiertcn_preference_loss, device, C.byref(r), C.byref(q))
     return dict(loss=loss, pair_loss=pair, margin=margin, seq_logp=seq, logp=logp, dlogits=dlogits)
 
@@ -94,17 +97,15 @@ def policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logp: torch.Tensor,
     if mean not in _MEAN:
         raise HierTCNError(f"mean {mean!r}: 'sequence' or 'token'")
     r, device, logp, dlogits, ws = _rows(logits, ids, grad_scale, want_grad, dlogits)
-    shape = (r.n, r.T)
+    shape = ids.shape
     need(old_logp, "old_logp", torch.float32, device, shape)
-    if isinstance(advantage, torch.Tensor) and advantage.dim() == 1:
-        advantage = advantage[:, None].expand(shape)
-    need(advantage, "advantage", torch.float32, device, shape, contiguous=False)
+    per_sequence = isinstance(advantage, torch.Tensor) and advantage.dim() == 1
+    need(advantage, "advantage", torch.float32, device, shape[:1] if per_sequence else shape, contiguous=False)
+    sn, st = (*advantage.stride(), 0)[:2]
     out = torch.empty(3, dtype=torch.float32, device=device)
     base = out.data_ptr()
-    q = _ops.Policy(mean=_MEAN[mean], clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef, old_logp=old_logp.data_ptr(), advantage=advantage.data_ptr(),
-                    adv_sn=advantage.stride(0), adv_st=advantage.stride(1), loss=base, kl=base + 4, clipped=base + 8)
-    if ref_logp is not None:
-        q.ref_logp = need(ref_logp, "ref_logp", torch.float32, device, shape).data_ptr()
+    ref = None if ref_logp is None else need(ref_logp, "ref_logp", torch.float32, device, shape).data_ptr()
+    q = _ops.Policy(_MEAN[mean], 0, clip_low, clip_high, kl_coef, old_logp.data_ptr(), ref, advantage.data_ptr(), sn, st, base, base + 4, base + 8)
     _ops.call(_ops.lib().hiertcn_policy_loss, device, C.byref(r), C.byref(q))
     loss, kl, clipped = out.unbind()
     return dict(loss=loss, kl=kl, clipped=clipped, logp=logp, dlogits=dlogits)

@@ -37,7 +37,7 @@ enum hiertcn_dtype { HIERTCN_FP32 = 0, HIERTCN_BF16 = 1, HIERTCN_FP16 = 2 };
  * mask: the user-boundary reset of model_hier.py:93 (0 cuts the state whatever it holds, NaN included; anything else keeps it).  lengths: dynamic_rnn's
  * sequence_length (model_gru.py:47-53): behind it the output is 0 and the state is carried; gate, cand and dout are not read there.  Values below 0
  * and above T count as 0 and T.  States are fp32; out is rounded once to dtype.
- *   record   needed by the backward pass: the state before every 8th step (hiertcn_glr_record_floats floats), written by the forward pass when non-NULL
+ *   record   needed by the backward pass: the state before every 16th step (hiertcn_glr_record_floats floats), written by the forward pass when non-NULL
  *   backward lambda_t = dout_t + a_{t+1} lambda_{t+1} with a = u [mask != 0] and dstate_out entering behind the last step;
  *            dcand = lambda (1 - u) act'(cand), dgate = lambda (h_prev - c) u (1 - u), dstate_in = a_0 lambda_0; rows behind lengths[b] get 0
  * state_out may be state_in itself.  Other outputs overlap neither each other nor inputs (refused where it can be seen from pointers and strides).
