@@ -10,8 +10,8 @@
 // Where there are few sequences for the machine the tiles of a sequence go to different workgroups (CHAIN).  A workgroup publishes its tile's map, applies
 // those of the tiles before it in its group of 16 to the state before the group, and the last of a group publishes the state behind it.  The order of
 // all that is the order of time, whoever waits for whom, so results do not depend on timing.  A word (A, S) is its own flag: 64 bits, written by one store that
-// goes past the L2s, all ones until then (a NaN is stored as the canonical one, so that no result looks like that).  A workgroup waits for workgroups of lower
-// TICKETS only, tickets are drawn at the start of a workgroup, and the one with the lowest ticket waits for nobody: every wait ends.
+// goes past the L2s, all ones until then (a NaN is stored as the canonical one, so that no result looks like that).  A workgroup takes the tile of its TICKET, drawn
+// when it starts, and waits for lower tickets only: those run, and the lowest waits for nobody, so every wait ends, however workgroups are dispatched.
 //
 // The backward pass is the same recurrence the other way round, lambda_t = dout_t + a_{t+1} lambda_{t+1}: with r_t = a_t lambda_t a run maps r -> A r + Q
 // with the same A.  States are not read back from the rounded output: the forward pass leaves the fp32 state before every segment in `record`, 1/16 of
@@ -39,7 +39,6 @@ struct GlrP {
   unsigned* ticket;
 };
 constexpr int GROUP = 16;        // tiles of a group
-constexpr uint64_t NOTHING = ~0ull;
 
 // maps: composition and application.  CUT: A = 0 marks a reset
 template <bool CUT>
@@ -103,7 +102,7 @@ struct Place {
     w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     nw = blockDim.x >> 6;
     const unsigned per = (unsigned)p.ncb * (unsigned)p.a.B;      // (the grid fits 31 bits)
-    tile = blk / per;
+    tile = (int)(blk / per);
     const unsigned rest = blk % per;
     b = rest / (unsigned)p.ncb;
     ch0 = (int64_t)(rest % (unsigned)p.ncb) * 64 * VEC;
@@ -207,27 +206,6 @@ __device__ __forceinline__ void tile_scan(float2* lds, const Place<VEC>& at, con
 }
 
 // ---- CHAIN ------------------------------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint64_t word(float lo, float hi) {
-  if (lo != lo) lo = __builtin_bit_cast(float, 0x7fc00000u);
-  return (uint64_t)__builtin_bit_cast(uint32_t, hi) << 32 | __builtin_bit_cast(uint32_t, lo);
-}
-__device__ __forceinline__ float low(uint64_t v) { return __builtin_bit_cast(float, (uint32_t)v); }
-__device__ __forceinline__ float high(uint64_t v) { return __builtin_bit_cast(float, (uint32_t)(v >> 32)); }
-__device__ __forceinline__ void publish(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ uint64_t look(const uint64_t* p) { return __hip_atomic_load(const_cast<uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
-// the ticket of the workgroup
-__device__ __forceinline__ unsigned draw(const GlrP& p, unsigned* place) {
-  if (threadIdx.x == 0) *place = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  return (unsigned)__builtin_amdgcn_readfirstlane((int)*place);
-}
-// Waits for a word.  (Its workgroup has a lower ticket: it runs, and waits for lower ones only.)
-__device__ __forceinline__ uint64_t await(const uint64_t* p) {
-  uint64_t v;
-  while ((v = look(p)) == NOTHING) __builtin_amdgcn_s_sleep(1);
-  return v;
-}
 // What a chained workgroup keeps in LDS: the maps of its waves, those of the tiles before it in its group, the state before the group, the ticket.
 template <int VEC>
 struct ChainLds {
@@ -262,19 +240,19 @@ __device__ __forceinline__ void chain_scan(const GlrP& p, const ChainLds<VEC>& l
       for (int i = 0; i < VEC; i++) tA[i] = map_a<CUT>(tA[i], lds.waves[(q * VEC + i) * 64 + lane].x);
     if (at.chan && place + 1 < GROUP)
 #pragma unroll
-      for (int i = 0; i < VEC; i++) publish(p.map + (int64_t)at.tile * plane + row + at.off + i, word(tS[i], tA[i]));
+      for (int i = 0; i < VEC; i++) ops_publish(p.map + (int64_t)at.tile * plane + row + at.off + i, ops_word(tS[i], tA[i]));
   }
   for (int q = at.w; q < place; q += at.nw)
 #pragma unroll
     for (int i = 0; i < VEC; i++) {
-      const uint64_t v = await(p.map + (int64_t)(group * GROUP + q) * plane + row + at.off + i);
-      lds.tiles[(q * VEC + i) * 64 + lane] = make_float2(high(v), low(v));
+      const uint64_t v = ops_await(p.map + (int64_t)(group * GROUP + q) * plane + row + at.off + i);
+      lds.tiles[(q * VEC + i) * 64 + lane] = make_float2(ops_high(v), ops_low(v));
     }
   if (at.w == at.nw - 1) {
     float f[VEC];
     if (group == 0) get_state<VEC>(p.state0, row, at, f);
 #pragma unroll
-    for (int i = 0; i < VEC; i++) lds.first[i * 64 + lane] = group == 0 ? f[i] : low(await(p.behind + (int64_t)(group - 1) * plane + row + at.off + i));
+    for (int i = 0; i < VEC; i++) lds.first[i * 64 + lane] = group == 0 ? f[i] : ops_low(ops_await(p.behind + (int64_t)(group - 1) * plane + row + at.off + i));
   }
   __syncthreads();
 #pragma unroll
@@ -293,14 +271,14 @@ __device__ __forceinline__ void chain_scan(const GlrP& p, const ChainLds<VEC>& l
   }
   if (at.w == 0 && at.chan && place + 1 == GROUP && at.tile + 1 < p.ntile)
 #pragma unroll
-    for (int i = 0; i < VEC; i++) publish(p.behind + (int64_t)group * plane + row + at.off + i, word(map_s<CUT>(tA[i], carry[i], tS[i]), 0.f));
+    for (int i = 0; i < VEC; i++) ops_publish(p.behind + (int64_t)group * plane + row + at.off + i, ops_word(map_s<CUT>(tA[i], carry[i], tS[i]), 0.f));
   fold_waves<VEC, CUT, REV>(lds.waves, at, carry, h);
 }
 // clears what a chain's words start from
 __global__ __launch_bounds__(256) void k_chain_init(GlrP p, const float* first, int64_t words) {
   const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x, n = p.a.B * p.a.D;
   if (i0 == 0) *p.ticket = 0;
-  for (int64_t i = i0; i < words; i += (int64_t)gridDim.x * 256) p.map[i] = NOTHING;
+  for (int64_t i = i0; i < words; i += (int64_t)gridDim.x * 256) p.map[i] = OPS_NOTHING;
   for (int64_t i = i0; i < n; i += (int64_t)gridDim.x * 256) p.state0[i] = first ? first[i] : 0.f;
 }
 
@@ -310,7 +288,7 @@ __global__ __launch_bounds__(64 * MAXW / VEC) void k_glr(GlrP p) {
   extern __shared__ float2 lds[];          // 2 x [nw][VEC][64]; CHAIN: ChainLds
   const hiertcn_glr_t& a = p.a;
   const ChainLds<VEC> chain(lds);
-  const Place<VEC> at(p, CHAIN ? draw(p, chain.ticket) : blockIdx.x);
+  const Place<VEC> at(p, CHAIN ? ops_ticket(p.ticket, chain.ticket) : blockIdx.x);
   const int64_t row = at.b * a.D + at.ch0;
   const int len = length_of(a, at.b), seg0 = CHAIN ? at.tile * at.nw : 0, seg1 = CHAIN && seg0 + at.nw < p.nseg ? seg0 + at.nw : p.nseg;
   float carry[VEC], h[VEC], u[SEG][VEC], s[SEG][VEC], A[VEC], S[VEC];
@@ -386,7 +364,7 @@ __global__ __launch_bounds__(64 * MAXW) void k_glr_bwd(GlrP p) {
   extern __shared__ float2 lds[];          // as in k_glr
   const hiertcn_glr_t& a = p.a;
   const ChainLds<VEC> chain(lds);
-  const Place<VEC> at(p, CHAIN ? draw(p, chain.ticket) : blockIdx.x);
+  const Place<VEC> at(p, CHAIN ? ops_ticket(p.ticket, chain.ticket) : blockIdx.x);
   const int64_t row = at.b * a.D + at.ch0;
   const int len = length_of(a, at.b), seg0 = CHAIN ? (p.ntile - 1 - at.tile) * at.nw : 0, seg1 = CHAIN && seg0 + at.nw < p.nseg ? seg0 + at.nw : p.nseg;
   const int tiles = (seg1 - seg0 + at.nw - 1) / at.nw;
@@ -488,7 +466,7 @@ Plan plan_of(int64_t B, int64_t T, int64_t D, bool wide, bool backward) {
   return q;
 }
 int64_t words_of(const Plan& q, int64_t B, int64_t D) { return (q.ntile + q.ntile / GROUP + 1) * B * D; }
-size_t bytes_of(const Plan& q, int64_t B, int64_t D) { return q.chain ? (size_t)words_of(q, B, D) * 8 + (size_t)(B * D) * 4 + 16 : 0; }
+size_t bytes_of(const Plan& q, int64_t B, int64_t D) { return q.chain ? (size_t)words_of(q, B, D) * 8 + (size_t)(B * D) * 4 + 256 : 0; }
 
 size_t workspace_of(int64_t B, int64_t T, int64_t D) {
   size_t most = 0;
@@ -615,7 +593,7 @@ int glr(const hiertcn_glr_t* in, bool backward, hipStream_t st) {
     p.map = static_cast<uint64_t*>(a.workspace);
     p.behind = p.map + q.ntile * a.B * a.D;
     p.state0 = reinterpret_cast<float*>(p.map + words_of(q, a.B, a.D));
-    p.ticket = reinterpret_cast<unsigned*>(p.state0 + a.B * a.D);
+    p.ticket = reinterpret_cast<unsigned*>(p.state0 + (a.B * a.D + 31) / 32 * 32);
   }
   OPS_TRY(a.dtype == HIERTCN_FP32 ? go_vec<HIERTCN_FP32>(p, q, backward, st) : a.dtype == HIERTCN_BF16 ? go_vec<HIERTCN_BF16>(p, q, backward, st) : go_vec<HIERTCN_FP16>(p, q, backward, st));
   return HIERTCN_OK;

@@ -70,18 +70,25 @@ __device__ __forceinline__ void ops_ld(const void* __restrict__ p, int64_t off, 
     for (int i = 0; i < VEC; i++) o[i] = ops_h2f(x.v[i], DT);
   }
 }
-template <int DT, int VEC>
+typedef float ops_f4 __attribute__((ext_vector_type(4)));
+template <bool PAST, typename T>
+__device__ __forceinline__ void ops_put(void* p, const T& x) {
+  if constexpr (PAST && sizeof(T) == 16) __builtin_nontemporal_store(__builtin_bit_cast(ops_f4, x), static_cast<ops_f4*>(p));
+  else *static_cast<T*>(p) = x;
+}
+// PAST: a store that leaves the caches to others, 16 bytes wide (and an ordinary one at any other width)
+template <int DT, int VEC, bool PAST = false>
 __device__ __forceinline__ void ops_st(void* __restrict__ p, int64_t off, const float (&o)[VEC]) {
   if constexpr (DT == HIERTCN_FP32) {
     OpsF<VEC> x;
 #pragma unroll
     for (int i = 0; i < VEC; i++) x.v[i] = o[i];
-    *reinterpret_cast<OpsF<VEC>*>(static_cast<float*>(p) + off) = x;
+    ops_put<PAST>(static_cast<float*>(p) + off, x);
   } else {
     OpsH<VEC> x;
 #pragma unroll
     for (int i = 0; i < VEC; i++) x.v[i] = ops_f2h(o[i], DT);
-    *reinterpret_cast<OpsH<VEC>*>(static_cast<uint16_t*>(p) + off) = x;
+    ops_put<PAST>(static_cast<uint16_t*>(p) + off, x);
   }
 }
 // the same in two steps, so that many loads can be in flight before the first is converted
@@ -96,6 +103,26 @@ __device__ __forceinline__ void ops_cvt(const typename OpsRaw<DT, VEC>::type& x,
     if constexpr (DT == HIERTCN_FP32) o[i] = x.v[i];
     else o[i] = ops_h2f(x.v[i], DT);
   }
+}
+// ---- words between workgroups: 64 bits that are their own flag, all ones until written; one store or load that goes past the L2s --------------------
+constexpr uint64_t OPS_NOTHING = ~0ull;
+__device__ __forceinline__ uint64_t ops_word(float lo, float hi) {      // (a NaN in the low half is stored as the canonical one: no result looks like nothing)
+  if (lo != lo) lo = __builtin_bit_cast(float, 0x7fc00000u);
+  return (uint64_t)__builtin_bit_cast(uint32_t, hi) << 32 | __builtin_bit_cast(uint32_t, lo);
+}
+__device__ __forceinline__ float ops_low(uint64_t v) { return __builtin_bit_cast(float, (uint32_t)v); }
+__device__ __forceinline__ float ops_high(uint64_t v) { return __builtin_bit_cast(float, (uint32_t)(v >> 32)); }
+__device__ __forceinline__ void ops_publish(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t ops_await(const uint64_t* p) {
+  uint64_t v;
+  while ((v = __hip_atomic_load(const_cast<uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == OPS_NOTHING) __builtin_amdgcn_s_sleep(1);
+  return v;
+}
+// The ticket of a workgroup: the order in which workgroups START, whatever order they are dispatched in.  `place`: LDS.  One barrier.
+__device__ __forceinline__ unsigned ops_ticket(unsigned* counter, unsigned* place) {
+  if (threadIdx.x == 0) *place = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return (unsigned)__builtin_amdgcn_readfirstlane((int)*place);
 }
 // 2^x through v_exp_f32 (one ulp); e^x for |x| that matter here
 __device__ __forceinline__ float ops_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }

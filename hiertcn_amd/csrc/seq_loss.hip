@@ -4,8 +4,8 @@
 //   dz_j = c (  [j = y] - exp(z_j - m) / s ),   c = d loss / d logp,
 // and a loss differs from another only in how c comes from the logp's.  Three launches:
 //   k_part    one pass over the logits: (m, s) of every part of every row, running maximum and sum
-//   k_pairs / k_policy / k_logp   joins a row's parts, forms logp, the loss and c
-//   k_dlogits one pass over the logits: dz  (its last workgroup adds up the loss)
+//   k_pairs / k_policy / k_logp   a few lanes a row: joins its parts, forms logp; the loss and c, in 64 bits (they are few)
+//   k_dlogits one pass over the logits: dz  (its first workgroup adds up the loss)
 // Masked rows are not read: their gradient rows are written as zeros.  All sums run in a fixed order.
 #include <math.h>
 
@@ -14,18 +14,26 @@
 namespace {
 
 constexpr int NT = 256;                 // threads of a workgroup
-constexpr int MAX_PARTS = 64;
+constexpr int MAX_PARTS = 64;           // a wave joins a row's parts, one to a lane
 
+// how a row is split over workgroups
+struct Cut {
+  int parts;
+  int64_t chunk;                        // vectors of a part
+  int tpr;                              // threads of a part: NT, or a wave (four rows to a workgroup) where a row has few vectors
+};
 struct RowsP {
   hiertcn_rows_t a;
   int64_t R;
-  int parts;
-  int64_t chunk;                        // vectors of a part
+  Cut read, write;                      // k_part's and k_dlogits'
   float2* part;                         // [R][parts] (m, s)
   float2* stat;                         // [R] (m, 1 / s)
   float* coef;                          // [R] d (grad_scale * loss) / d logp
-  float* term;                          // [3][R] policy: weighted loss, kl, clipped per row
+  double* term;                         // [3][groups] policy: weighted loss, kl, clipped of k_policy's workgroups
   int32_t* count;                       // [n] policy: answers of a sequence
+  int64_t* total;                       // [counters][2] policy: answers, sequences with answers, of the workgroups that count
+  int64_t groups, counters;
+  int lanes;                            // lanes of k_pairs / k_policy / k_logp that join a row's parts: a power of two
 };
 
 __device__ __forceinline__ bool answered(const hiertcn_rows_t& a, int64_t r, int32_t& y) {
@@ -45,160 +53,200 @@ __device__ __forceinline__ void wave_join(float& m, float& s) {
   for (int d = 32; d; d >>= 1) join(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
 }
 
-// the part of a row as [head] vectors [tail]: head elements up to the first address that a vector may be loaded from
+// the part of a row as [head] vectors [tail]: head elements up to the first address that a vector may be loaded from.  (V < 2^31: ints.)
 template <int DT, int VEC>
 struct Span {
-  int64_t head, nvec, v0, v1;           // v0 .. v1: this part's vectors; element of vector v: head + v * VEC
-  int64_t tail;                         // first element behind the vectors
-  __device__ Span(const void* row, int64_t V, int64_t chunk, int part) {
+  int head, v0, v1;                     // v0 .. v1: this part's vectors; element of vector v: head + v * VEC
+  int tail;                             // first element behind the vectors
+  __device__ Span(const void* row, int V, int chunk, int part) {
     constexpr int ES = DT == HIERTCN_FP32 ? 4 : 2;
-    head = VEC == 1 ? 0 : (int64_t)((16 - ((uintptr_t)row & 15)) & 15) / ES;
+    head = VEC == 1 ? 0 : (int)((16 - ((uintptr_t)row & 15)) & 15) / ES;
     if (head > V) head = V;
-    nvec = (V - head) / VEC;
+    const int nvec = (V - head) / VEC;
     tail = head + nvec * VEC;
     v0 = part * chunk;
-    v1 = v0 + chunk < nvec ? v0 + chunk : nvec;
+    v1 = nvec - v0 < chunk ? nvec : v0 + chunk;
+  }
+  // this thread's element in front of or behind the vectors, or -1 (there are at most VEC - 1 of each)
+  __device__ int edge(int V, int part, int parts, int tid) const {
+    if (part == 0 && tid < head) return tid;
+    if (part == parts - 1 && tid >= 32 && tail + (tid - 32) < V) return tail + (tid - 32);
+    return -1;
   }
 };
 template <int DT>
 __device__ __forceinline__ const void* row_of(const void* p, int64_t off) {
   return DT == HIERTCN_FP32 ? (const void*)(static_cast<const float*>(p) + off) : (const void*)(static_cast<const uint16_t*>(p) + off);
 }
-
 template <int DT, int VEC>
-__global__ __launch_bounds__(NT) void k_part(RowsP p) {
-  constexpr int U = 4;
+__device__ __forceinline__ typename OpsRaw<DT, VEC>::type raw_at(const void* row, int e) {
+  return *static_cast<const typename OpsRaw<DT, VEC>::type*>(row_of<DT>(row, e));
+}
+// which row and part this thread works on.  false: none
+__device__ __forceinline__ bool place_of(const RowsP& p, const Cut& c, unsigned wg, int tpr, int64_t& r, int& part, int& tid) {
+  tid = threadIdx.x & (tpr - 1);
+  if (tpr == NT) {
+    r = wg / (unsigned)c.parts;
+    part = (int)(wg % (unsigned)c.parts);
+  } else {                              // (one part)
+    r = (int64_t)wg * (NT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    part = 0;
+  }
+  return r < p.R;
+}
+
+// U vectors' share of a running (m, s)
+template <int DT, int VEC, int U>
+__device__ __forceinline__ void fold(const typename OpsRaw<DT, VEC>::type (&x)[U], int live, float& m, float& s) {
+  float z[U][VEC], top = m;
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    ops_cvt<DT, VEC>(x[u], z[u]);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) {
+      if (u >= live) z[u][i] = -INFINITY;
+      top = fmaxf(top, z[u][i]);
+    }
+  }
+  const float ref = ref_of(top);
+  s *= ops_exp(m - ref);
+  m = top;
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int i = 0; i < VEC; i++) s += ops_exp(z[u][i] - ref);
+}
+
+// answers per sequence, and this workgroup's share of their totals: a thread a sequence where sequences are short, else a wave
+constexpr int COUNT_T = 64;
+__device__ void count_answers(const RowsP& p, unsigned wg) {
   const hiertcn_rows_t& a = p.a;
-  if ((int64_t)blockIdx.x >= p.R * p.parts) {                  // policy: the answers of a sequence
-    const int64_t q = blockIdx.x - p.R * p.parts;
-    int c = 0;
-    for (int64_t t = threadIdx.x; t < a.T; t += NT) {
+  const int lane = threadIdx.x & 63;
+  const bool thread = a.T <= COUNT_T;
+  const int64_t q = thread ? (int64_t)wg * NT + threadIdx.x : (int64_t)wg * (NT / 64) + (threadIdx.x >> 6);
+  int c = 0;
+  if (q < a.n)
+    for (int64_t t = thread ? 0 : lane; t < a.T; t += thread ? 1 : 64) {
       int32_t y;
       c += answered(a, q * a.T + t, y);
     }
-    __shared__ int cs[NT / 64];
+  if (!thread)
 #pragma unroll
     for (int d = 32; d; d >>= 1) c += __shfl_xor(c, d);
-    if ((threadIdx.x & 63) == 0) cs[threadIdx.x >> 6] = c;
-    __syncthreads();
-    if (threadIdx.x == 0) p.count[q] = cs[0] + cs[1] + cs[2] + cs[3];
+  const bool owner = q < a.n && (thread || lane == 0);
+  if (owner) p.count[q] = c;
+  int64_t all = owner ? c : 0;
+  int some = owner && c > 0;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d), some += __shfl_xor(some, d);
+  __shared__ int64_t sums[NT / 64][2];
+  if (lane == 0) sums[threadIdx.x >> 6][0] = all, sums[threadIdx.x >> 6][1] = some;
+  __syncthreads();
+  if (threadIdx.x < 2) p.total[2 * wg + threadIdx.x] = sums[0][threadIdx.x] + sums[1][threadIdx.x] + sums[2][threadIdx.x] + sums[3][threadIdx.x];
+}
+
+template <int DT, int VEC, int TPR>
+__global__ __launch_bounds__(NT) void k_part(RowsP p) {
+  constexpr int U = 4;
+  const hiertcn_rows_t& a = p.a;
+  if (blockIdx.x < p.counters) {
+    count_answers(p, blockIdx.x);
     return;
   }
-  const int64_t r = blockIdx.x / p.parts;
-  const int part = (int)(blockIdx.x % p.parts);
+  int64_t r;
+  int part, tid;
   int32_t y;
-  if (!answered(a, r, y)) return;
+  if (!place_of(p, p.read, blockIdx.x - (unsigned)p.counters, TPR, r, part, tid) || !answered(a, r, y)) return;
   const void* row = row_of<DT>(a.logits, r * a.ld);
-  const Span<DT, VEC> sp(row, a.V, p.chunk, part);
+  const Span<DT, VEC> sp(row, (int)a.V, (int)p.read.chunk, part);
   float m = -INFINITY, s = 0.f;
-  for (int64_t v = sp.v0 + threadIdx.x; v < sp.v1; v += NT * U) {
-    float z[U][VEC], top = -INFINITY;
+  typename OpsRaw<DT, VEC>::type x[U];
+  int v = sp.v0 + tid;
+  const int full = sp.v1 > sp.v0 ? (sp.v1 - sp.v0) / (TPR * U) : 0;
+  for (int k = 0; k < full; k++, v += TPR * U) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (v + u * NT < sp.v1) ops_ld<DT, VEC>(row, sp.head + (v + u * NT) * VEC, z[u]);
-      else
-#pragma unroll
-        for (int i = 0; i < VEC; i++) z[u][i] = -INFINITY;
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int i = 0; i < VEC; i++) top = fmaxf(top, z[u][i]);
-    top = fmaxf(top, m);
-    const float ref = ref_of(top);
-    s *= ops_exp(m - ref);
-    m = top;
-#pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int i = 0; i < VEC; i++) s += ops_exp(z[u][i] - ref);
+    for (int u = 0; u < U; u++) x[u] = raw_at<DT, VEC>(row, sp.head + (v + u * TPR) * VEC);
+    fold<DT, VEC, U>(x, U, m, s);
   }
-  // the elements in front of and behind the vectors
-  int64_t e = -1;
-  if (part == 0 && threadIdx.x < sp.head) e = threadIdx.x;
-  if (part == p.parts - 1 && threadIdx.x >= 32 && sp.tail + (threadIdx.x - 32) < a.V) {
-    e = sp.tail + (threadIdx.x - 32);
+  if (v < sp.v1) {                                             // the rest: addresses behind it are clamped, their values not taken
+    const int live = (sp.v1 - v + TPR - 1) / TPR;
+#pragma unroll
+    for (int u = 0; u < U; u++) x[u] = raw_at<DT, VEC>(row, sp.head + (u < live ? v + u * TPR : v) * VEC);
+    fold<DT, VEC, U>(x, live, m, s);
   }
+  const int e = sp.edge((int)a.V, part, p.read.parts, tid);
   if (e >= 0) {
     float z[1];
     ops_ld<DT, 1>(row, e, z);
     join(m, s, z[0], z[0] == -INFINITY ? 0.f : ops_exp(z[0] - z[0]));
   }
-  __shared__ float ms[NT / 64], ss[NT / 64];
   wave_join(m, s);
-  if ((threadIdx.x & 63) == 0) ms[threadIdx.x >> 6] = m, ss[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < NT / 64; w++) join(m, s, ms[w], ss[w]);
-    p.part[r * p.parts + part] = make_float2(m, s);
+  if constexpr (TPR == NT) {
+    __shared__ float ms[NT / 64], ss[NT / 64];
+    if ((threadIdx.x & 63) == 0) ms[threadIdx.x >> 6] = m, ss[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0)
+      for (int w = 1; w < NT / 64; w++) join(m, s, ms[w], ss[w]);
   }
+  if (tid == 0) p.part[r * p.read.parts + part] = make_float2(m, s);
 }
 
 __device__ __forceinline__ float logit(const hiertcn_rows_t& a, int64_t off) {
   return a.dtype == HIERTCN_FP32 ? static_cast<const float*>(a.logits)[off] : ops_h2f(static_cast<const uint16_t*>(a.logits)[off], a.dtype);
 }
 
-// logp of a row from its parts; (m, 1 / s) kept for the gradient.  false: masked, or nothing but -inf
-__device__ bool finish_row(const RowsP& p, int64_t r, float& logp) {
-  const hiertcn_rows_t& a = p.a;
+// p.lanes neighbours a row: logp from its parts, (m, 1 / s) kept for the gradient.  false: masked, or nothing but -inf
+__device__ bool finish_row(const RowsP& p, int64_t r, double& logp) {
   int32_t y;
-  logp = 0.f;
-  if (!answered(a, r, y)) return false;
-  float m = -INFINITY, s = 0.f;
-  for (int q = 0; q < p.parts; q++) {
-    const float2 x = p.part[r * p.parts + q];
-    join(m, s, x.x, x.y);
-  }
-  p.stat[r] = make_float2(m, 1.f / s);
+  logp = 0.0;
+  if (!answered(p.a, r, y)) return false;
+  const int i = threadIdx.x & (p.lanes - 1);
+  const float2 x = i < p.read.parts ? p.part[r * p.read.parts + i] : make_float2(-INFINITY, 0.f);
+  const float z = logit(p.a, r * p.a.ld + y);
+  float m = x.x, s = x.y;
+  for (int d = p.lanes >> 1; d; d >>= 1) join(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
+  if (i == 0) p.stat[r] = make_float2(m, 1.f / s);
   if (m == -INFINITY && s == 0.f) return false;
-  logp = (logit(a, r * a.ld + y) - ref_of(m)) - logf(s);
+  logp = ((double)z - ref_of(m)) - log((double)s);
   return true;
 }
+// the row of this thread's lanes, of n rows beginning at the workgroup's first
+__device__ __forceinline__ int64_t row_here(const RowsP& p) { return (int64_t)blockIdx.x * (NT / p.lanes) + threadIdx.x / p.lanes; }
+__device__ __forceinline__ bool first_lane(const RowsP& p) { return (threadIdx.x & (p.lanes - 1)) == 0; }
 
 __global__ __launch_bounds__(NT) void k_logp(RowsP p) {
-  const int64_t r = (int64_t)blockIdx.x * NT + threadIdx.x;
+  const int64_t r = row_here(p);
   if (r >= p.R) return;
-  float lp;
+  double lp;
   finish_row(p, r, lp);
-  p.a.logp[r] = lp;
+  if (first_lane(p)) p.a.logp[r] = (float)lp;
 }
 
-__device__ double block_sum(double x) {
-  __shared__ double t[NT / 64];
+// sums over a workgroup of W waves, for all its threads
+template <int W, int N>
+__device__ void block_sum(double (&x)[N]) {
+  __shared__ double t[W][N];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  for (int k = 0; k < N; k++)
+#pragma unroll
+    for (int d = 32; d; d >>= 1) x[k] += __shfl_xor(x[k], d);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) t[threadIdx.x >> 6] = x;
+#pragma unroll
+  for (int k = 0; k < N; k++)
+    if ((threadIdx.x & 63) == 0) t[threadIdx.x >> 6][k] = x[k];
   __syncthreads();
-  return t[0] + t[1] + t[2] + t[3];
+#pragma unroll
+  for (int k = 0; k < N; k++) {
+    x[k] = t[0][k];
+#pragma unroll
+    for (int w = 1; w < W; w++) x[k] += t[w][k];
+  }
 }
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
 
-// a workgroup a pair: both sums, the loss, the slope d loss / d s
-__global__ __launch_bounds__(NT) void k_pairs(RowsP p, hiertcn_preference_t q) {
-  const hiertcn_rows_t& a = p.a;
-  const int64_t P = a.n / 2;
-  double s[2];
-  double cnt[2];
-  for (int side = 0; side < 2; side++) {
-    const int64_t seq = blockIdx.x + side * P;
-    double sum = 0.0, c = 0.0;
-    for (int64_t t = threadIdx.x; t < a.T; t += NT) {
-      const int64_t r = seq * a.T + t;
-      float lp;
-      const bool live = finish_row(p, r, lp);
-      a.logp[r] = lp;
-      int32_t y;
-      c += answered(a, r, y);
-      p.coef[r] = live ? 1.f : 0.f;
-      sum += lp;
-    }
-    sum = block_sum(sum);
-    cnt[side] = block_sum(c);
-    s[side] = q.average ? (cnt[side] > 0 ? sum / cnt[side] : 0.0) : sum;
-  }
-  const double beta = q.beta, eps = q.smoothing, D = (s[0] - q.ref[blockIdx.x]) - (s[1] - q.ref[blockIdx.x + P]);
-  double loss, slope;
+// loss and d loss / d D of a pair
+__device__ __forceinline__ void pair_of(const hiertcn_preference_t& q, double D, double& loss, double& slope) {
+  const double beta = q.beta, eps = q.smoothing;
   if (q.kind == 0) {
     loss = (1.0 - eps) * softplus(-beta * D) + (eps > 0.0 ? eps * softplus(beta * D) : 0.0);
     slope = beta * (1.0 / (1.0 + exp(-beta * D)) - (1.0 - eps));
@@ -210,121 +258,181 @@ __global__ __launch_bounds__(NT) void k_pairs(RowsP p, hiertcn_preference_t q) {
     loss = off * off;
     slope = 2.0 * off;
   }
-  if (threadIdx.x == 0) {
+}
+// c of a sequence's rows, from the pair's slope
+__device__ __forceinline__ float coef_of(const RowsP& p, const hiertcn_preference_t& q, double slope, int side, double count) {
+  return (float)((side ? -slope : slope) / (double)(p.a.n / 2) * p.a.grad_scale / (q.average && count > 0 ? count : 1.0));
+}
+
+// a workgroup a pair: both sums, the loss, the rows' c.  (A thousand threads: the rows are a few hundred loads, one behind the other in a thread.)
+constexpr int PAIR_NT = 1024;
+__global__ __launch_bounds__(PAIR_NT) void k_pairs(RowsP p, hiertcn_preference_t q) {
+  const hiertcn_rows_t& a = p.a;
+  const int64_t P = a.n / 2;
+  const int64_t first = threadIdx.x / p.lanes, step = PAIR_NT / p.lanes;
+  double x[4] = {};                                            // sums of logp, numbers of answers
+  for (int64_t i = first; i < 2 * a.T; i += step) {
+    const int side = i >= a.T;
+    const int64_t r = side ? (blockIdx.x + P) * a.T + (i - a.T) : blockIdx.x * a.T + i;
+    double lp;
+    const bool live = finish_row(p, r, lp);
+    if (first_lane(p)) {
+      int32_t y;
+      a.logp[r] = (float)lp;
+      p.coef[r] = live ? 1.f : 0.f;
+      const double one = answered(a, r, y) ? 1.0 : 0.0;
+      x[0] += side ? 0.0 : lp;
+      x[1] += side ? lp : 0.0;
+      x[2] += side ? 0.0 : one;
+      x[3] += side ? one : 0.0;
+    }
+  }
+  block_sum<PAIR_NT / 64>(x);
+  double s[2];
+  for (int side = 0; side < 2; side++) s[side] = q.average ? (x[2 + side] > 0 ? x[side] / x[2 + side] : 0.0) : x[side];
+  __shared__ float c[2];
+  if (threadIdx.x == 0) {                                      // one wave: 64-bit exponentials in all 16 cost 5 us
+    const double D = (s[0] - q.ref[blockIdx.x]) - (s[1] - q.ref[blockIdx.x + P]);
+    double loss, slope;
+    pair_of(q, D, loss, slope);
+    c[0] = coef_of(p, q, slope, 0, x[2]);
+    c[1] = coef_of(p, q, slope, 1, x[3]);
     q.pair_loss[blockIdx.x] = (float)loss;
     q.margin[blockIdx.x] = (float)D;
     q.seq_logp[blockIdx.x] = (float)s[0];
     q.seq_logp[blockIdx.x + P] = (float)s[1];
   }
-  for (int side = 0; side < 2; side++) {
-    const int64_t seq = blockIdx.x + side * P;
-    const double c = (side ? -slope : slope) / (double)P * a.grad_scale / (q.average ? (cnt[side] > 0 ? cnt[side] : 1.0) : 1.0);
-    for (int64_t t = threadIdx.x; t < a.T; t += NT) {        // (this thread's own rows of the loop above)
-      const int64_t r = seq * a.T + t;
-      p.coef[r] = p.coef[r] != 0.f ? (float)c : 0.f;
-    }
+  __syncthreads();
+  if (!first_lane(p)) return;
+  for (int64_t i = first; i < 2 * a.T; i += step) {            // (this thread's own rows of the loop above)
+    const int side = i >= a.T;
+    const int64_t r = side ? (blockIdx.x + P) * a.T + (i - a.T) : blockIdx.x * a.T + i;
+    p.coef[r] = p.coef[r] != 0.f ? c[side] : 0.f;
   }
 }
 
-// a thread a row
+// one answer of the policy loss: its weighted loss, kl and [clipped], and c without grad_scale
+struct Answer { double loss, kl, cut, c; };
+__device__ __forceinline__ Answer answer_of(const hiertcn_policy_t& q, int64_t T, int64_t r, double lp, double weight) {
+  Answer o;
+  const double A = q.advantage[r / T * q.adv_sn + r % T * q.adv_st];
+  const double ratio = exp(lp - q.old_logp[r]);
+  const double lo = 1.0 - q.clip_low, hi = 1.0 + q.clip_high;
+  const double bounded = ratio < lo ? lo : ratio > hi ? hi : ratio;
+  const double none = lp != lp ? lp : 0.0;      // 0, or the NaN of the row
+  const double x = A == 0.0 ? none : ratio * A, y = A == 0.0 ? none : bounded * A;
+  const bool clipped = x > y;
+  o.loss = clipped ? -y : -x;
+  o.cut = clipped ? weight : 0.0;
+  o.c = clipped ? none : -x;
+  o.kl = 0.0;
+  if (q.ref_logp) {
+    const double gap = q.ref_logp[r] - lp, e = expm1(gap);
+    o.kl = e == INFINITY ? e : e - gap;
+    o.loss += q.kl_coef * o.kl;
+    o.c += q.kl_coef * -e;
+  }
+  o.loss *= weight;
+  o.kl *= weight;
+  o.c *= weight;
+  return o;
+}
+
 __global__ __launch_bounds__(NT) void k_policy(RowsP p, hiertcn_policy_t q) {
   const hiertcn_rows_t& a = p.a;
-  double total = 0.0;                    // sequences with answers, or answers
-  for (int64_t i = threadIdx.x; i < a.n; i += NT) total += q.mean == 0 ? (p.count[i] > 0 ? 1.0 : 0.0) : (double)p.count[i];
-  total = block_sum(total);
-  const int64_t r = (int64_t)blockIdx.x * NT + threadIdx.x;
-  if (r >= p.R) return;
-  const int64_t b = r / a.T, t = r % a.T;
-  float lp;
-  const bool live = finish_row(p, r, lp);
-  a.logp[r] = lp;
-  float loss = 0.f, kl = 0.f, cut = 0.f, c = 0.f;
-  if (live) {
-    const float weight = (float)(1.0 / (q.mean == 0 ? total * p.count[b] : total));
-    const float A = q.advantage[b * q.adv_sn + t * q.adv_st];
-    const float ratio = expf(lp - q.old_logp[r]);
-    const float lo = 1.f - q.clip_low, hi = 1.f + q.clip_high;
-    const float held = ratio < lo ? lo : ratio > hi ? hi : ratio;
-    const float none = lp != lp ? lp : 0.f;       // 0, or the NaN of the row
-    const float x = A == 0.f ? none : ratio * A, y = A == 0.f ? none : held * A;
-    const bool clipped = x > y;
-    loss = clipped ? -y : -x;
-    cut = clipped ? weight : 0.f;
-    c = clipped ? none : -x;
-    if (q.ref_logp) {
-      const float gap = q.ref_logp[r] - lp, e = expf(gap);
-      kl = e == INFINITY ? e : (e - gap) - 1.f;
-      if (fabsf(gap) < 0.25f)            // e^gap - gap - 1 loses its digits there: the series
-        kl = gap * gap * fmaf(gap, fmaf(gap, fmaf(gap, fmaf(gap, fmaf(gap, 1.f / 5040.f, 1.f / 720.f), 1.f / 120.f), 1.f / 24.f), 1.f / 6.f), 0.5f);
-      loss += q.kl_coef * kl;
-      c += q.kl_coef * -expm1f(gap);
+  double total[1] = {};                                        // sequences with answers, or answers
+  for (int64_t i = threadIdx.x; i < p.counters; i += NT) total[0] += (double)p.total[2 * i + (q.mean == 0)];
+  block_sum<NT / 64>(total);
+  const int64_t r = row_here(p);
+  double x[3] = {};
+  if (r < p.R) {
+    double lp;
+    const bool live = finish_row(p, r, lp);
+    if (first_lane(p)) {
+      Answer o{0.0, 0.0, 0.0, 0.0};
+      if (live) o = answer_of(q, a.T, r, lp, 1.0 / (q.mean == 0 ? total[0] * p.count[r / a.T] : total[0]));
+      a.logp[r] = (float)lp;
+      p.coef[r] = (float)(o.c * a.grad_scale);
+      x[0] = o.loss, x[1] = o.kl, x[2] = o.cut;
     }
-    loss *= weight;
-    kl *= weight;
-    c *= weight * a.grad_scale;
   }
-  p.coef[r] = c;
-  p.term[r] = loss;
-  p.term[p.R + r] = kl;
-  p.term[2 * p.R + r] = cut;
+  block_sum<NT / 64>(x);
+  if (threadIdx.x < 3) p.term[threadIdx.x * p.groups + blockIdx.x] = threadIdx.x == 0 ? x[0] : threadIdx.x == 1 ? x[1] : x[2];
 }
 
-// out[k] = scale * sum of src[k * n ..], one workgroup
-struct Sums { const float* src; int64_t n; float scale; float* out[3]; };
+// out[k] = scale * sum of a row of n numbers, one workgroup
+struct Sums { const float* f; const double* d; int64_t n; double scale; float* out[3]; };
 __device__ void add_up(const Sums& q) {
-  for (int k = 0; k < 3; k++) {
-    if (!q.out[k]) continue;
-    double x = 0.0;
-    for (int64_t i = threadIdx.x; i < q.n; i += NT) x += q.src[k * q.n + i];
-    x = block_sum(x);
-    if (threadIdx.x == 0) q.out[k][0] = (float)(x * q.scale);
+  double x[3] = {};
+  for (int64_t i = threadIdx.x; i < q.n; i += NT) {
+    if (q.f) x[0] += q.f[i];
+    else
+#pragma unroll
+      for (int k = 0; k < 3; k++) x[k] += q.d[k * q.n + i];
   }
+  block_sum<NT / 64>(x);
+#pragma unroll
+  for (int k = 0; k < 3; k++)
+    if (threadIdx.x == 0 && q.out[k]) q.out[k][0] = (float)(x[k] * q.scale);
 }
 __global__ __launch_bounds__(NT) void k_sums(Sums q) { add_up(q); }
 
 template <int DT, int VEC>
+__device__ __forceinline__ void gradient_of(const typename OpsRaw<DT, VEC>::type& x, void* out, int at, float ref, float g, float c, int y) {
+  float z[VEC];
+  ops_cvt<DT, VEC>(x, z);
+#pragma unroll
+  for (int i = 0; i < VEC; i++) z[i] = g * ops_exp(z[i] - ref);
+  if (y >= at && y - at < VEC)
+#pragma unroll
+    for (int i = 0; i < VEC; i++) z[i] += i == y - at ? c : 0.f;
+  ops_st<DT, VEC, true>(out, at, z);
+}
+
+template <int DT, int VEC, int TPR>
 __global__ __launch_bounds__(NT) void k_dlogits(RowsP p, Sums q) {
   constexpr int U = 4;
   const hiertcn_rows_t& a = p.a;
-  if ((int64_t)blockIdx.x >= p.R * p.parts) {
+  if (blockIdx.x == 0) {
     add_up(q);
     return;
   }
-  const int64_t r = blockIdx.x / p.parts;
-  const int part = (int)(blockIdx.x % p.parts);
+  int64_t r;
+  int part, tid;
+  // backwards: k_part's last rows may still be in the last level of cache.  Its lines are not kept for the stores' sake (64 x 30 x 300000 bf16, both
+  // passes: 546 us; stores past the caches 520, backwards 525, both 501)
+  if (!place_of(p, p.write, gridDim.x - 1 - blockIdx.x, TPR, r, part, tid)) return;
+  const float c = p.coef[r];
+  const float2 st = p.stat[r];                                 // (not written for a masked row, and not used)
+  const int y = a.ids[r];
   const void* row = row_of<DT>(a.logits, r * a.ld);
   void* out = const_cast<void*>(row_of<DT>(a.dlogits, r * a.dld));
-  const Span<DT, VEC> sp(out, a.V, p.chunk, part);
-  const float c = p.coef[r];
-  int64_t e = -1;
-  if (part == 0 && threadIdx.x < sp.head) e = threadIdx.x;
-  if (part == p.parts - 1 && threadIdx.x >= 32 && sp.tail + (threadIdx.x - 32) < a.V) e = sp.tail + (threadIdx.x - 32);
+  const Span<DT, VEC> sp(out, (int)a.V, (int)p.write.chunk, part);
+  const int e = sp.edge((int)a.V, part, p.write.parts, tid);
+  int v = sp.v0 + tid;
   if (c == 0.f) {
     const float zero[VEC] = {};
-    for (int64_t v = sp.v0 + threadIdx.x; v < sp.v1; v += NT) ops_st<DT, VEC>(out, sp.head + v * VEC, zero);
+    for (; v < sp.v1; v += TPR) ops_st<DT, VEC, true>(out, sp.head + v * VEC, zero);
     const float z1[1] = {0.f};
     if (e >= 0) ops_st<DT, 1>(out, e, z1);
     return;
   }
-  const int32_t y = a.ids[r];
-  const float2 st = p.stat[r];
   const float ref = ref_of(st.x), g = -c * st.y;
-  for (int64_t v = sp.v0 + threadIdx.x; v < sp.v1; v += NT * U) {
-    float z[U][VEC];
+  typename OpsRaw<DT, VEC>::type x[U];
+  const int full = sp.v1 > sp.v0 ? (sp.v1 - sp.v0) / (TPR * U) : 0;
+  for (int k = 0; k < full; k++, v += TPR * U) {
+#pragma unroll
+    for (int u = 0; u < U; u++) x[u] = raw_at<DT, VEC>(row, sp.head + (v + u * TPR) * VEC);
+#pragma unroll
+    for (int u = 0; u < U; u++) gradient_of<DT, VEC>(x[u], out, sp.head + (v + u * TPR) * VEC, ref, g, c, y);
+  }
+  if (v < sp.v1) {
+    const int live = (sp.v1 - v + TPR - 1) / TPR;
+#pragma unroll
+    for (int u = 0; u < U; u++) x[u] = raw_at<DT, VEC>(row, sp.head + (u < live ? v + u * TPR : v) * VEC);
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (v + u * NT < sp.v1) ops_ld<DT, VEC>(row, sp.head + (v + u * NT) * VEC, z[u]);
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (v + u * NT >= sp.v1) break;
-      const int64_t at = sp.head + (v + u * NT) * VEC;
-#pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        z[u][i] = g * ops_exp(z[u][i] - ref);
-        if (at + i == y) z[u][i] += c;
-      }
-      ops_st<DT, VEC>(out, at, z[u]);
-    }
+      if (u < live) gradient_of<DT, VEC>(x[u], out, sp.head + (v + u * TPR) * VEC, ref, g, c, y);
   }
   if (e >= 0) {
     float z[1];
@@ -337,30 +445,45 @@ __global__ __launch_bounds__(NT) void k_dlogits(RowsP p, Sums q) {
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------------------
 size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
-int64_t chunk_of(int64_t V, int vec) {         // vectors of a part: 8192 elements, more where that would make over MAX_PARTS parts
-  int64_t elems = 8192;
+// parts of `elems` elements, or of as many more as MAX_PARTS asks for; a wave for a row that four rounds of a wave's loads cover
+Cut cut_of(int64_t V, int vec, int64_t elems) {
   if ((V + elems - 1) / elems > MAX_PARTS) elems = (V + MAX_PARTS - 1) / MAX_PARTS;
-  return (elems + vec - 1) / vec;
+  Cut c;
+  c.chunk = (elems + vec - 1) / vec;
+  const int64_t nvec = V / vec;
+  c.parts = (int)(nvec <= c.chunk ? 1 : (nvec + c.chunk - 1) / c.chunk);
+  c.tpr = nvec <= 256 ? 64 : NT;
+  return c;
 }
-int parts_of(int64_t V, int vec) {
-  const int64_t c = chunk_of(V, vec), nvec = V / vec;
-  return (int)(nvec <= c ? 1 : (nvec + c - 1) / c);
+constexpr int64_t PART = 8192;
+// k_part's parts grow while 8192 of them are left
+Cut read_of(int64_t R, int64_t V, int vec) {
+  int64_t elems = PART;
+  while (elems < 4 * PART && R * ((V + 2 * elems - 1) / (2 * elems)) >= 8192) elems *= 2;
+  return cut_of(V, vec, elems);
 }
+int64_t workgroups(const Cut& c, int64_t R) { return c.tpr == NT ? R * c.parts : (R + NT / 64 - 1) / (NT / 64); }
+int64_t counters_of(int64_t n, int64_t T) { return T <= COUNT_T ? (n + NT - 1) / NT : (n + NT / 64 - 1) / (NT / 64); }
 size_t workspace_of(int64_t n, int64_t T, int64_t V, RowsP* p) {
   const size_t R = (size_t)(n * T);
   int most = 1;
-  for (int vec : {1, 4, 8})
-    if (parts_of(V, vec) > most) most = parts_of(V, vec);
-  const size_t sizes[5] = {align_up(R * most * 8), align_up(R * 8), align_up(R * 4), align_up(R * 12), align_up((size_t)n * 4)};
+  for (int vec : {1, 4, 8}) most = most > read_of(n * T, V, vec).parts ? most : read_of(n * T, V, vec).parts;
+  int lanes = 1;
+  while (lanes < most) lanes *= 2;
+  const size_t groups = (R + NT / lanes - 1) / (NT / lanes);
+  const size_t sizes[6] = {align_up(R * most * 8), align_up(R * 8), align_up(R * 4), align_up(groups * 24), align_up((size_t)n * 4), align_up((size_t)counters_of(n, T) * 16)};
   if (p) {
     char* w = static_cast<char*>(p->a.workspace);
     p->part = reinterpret_cast<float2*>(w);
     p->stat = reinterpret_cast<float2*>(w += sizes[0]);
     p->coef = reinterpret_cast<float*>(w += sizes[1]);
-    p->term = reinterpret_cast<float*>(w += sizes[2]);
+    p->term = reinterpret_cast<double*>(w += sizes[2]);
     p->count = reinterpret_cast<int32_t*>(w += sizes[3]);
+    p->total = reinterpret_cast<int64_t*>(w += sizes[4]);
+    p->lanes = lanes;
+    p->groups = (int64_t)groups;
   }
-  return sizes[0] + sizes[1] + sizes[2] + sizes[3] + sizes[4];
+  return sizes[0] + sizes[1] + sizes[2] + sizes[3] + sizes[4] + sizes[5];
 }
 
 // the checks that all entries share; sets up p
@@ -392,23 +515,28 @@ int prepare(const hiertcn_rows_t* in, bool grad, RowsP& p, int& vec) {
   // 16 bytes at a time wherever the two passes' rows are 16-byte aligned alike; else one element
   vec = 16 / es;
   if (a.dlogits && (((uintptr_t)a.logits - (uintptr_t)a.dlogits) % 16 || (a.ld - a.dld) % vec)) vec = 1;
-  p.parts = parts_of(a.V, vec);
-  p.chunk = chunk_of(a.V, vec);
+  p.read = read_of(p.R, a.V, vec);
+  p.write = cut_of(a.V, vec, PART);
+  p.counters = 0;
   workspace_of(a.n, a.T, a.V, &p);
-  if (p.R * p.parts + a.n > 0x7fffffffll) return ops_fail(HIERTCN_ERR_INVALID, "n * T * V is too large for one launch");
+  if (workgroups(p.read, p.R) + a.n > 0x7fffffffll || workgroups(p.write, p.R) + a.n > 0x7fffffffll) return ops_fail(HIERTCN_ERR_INVALID, "n * T * V is too large for one launch");
   return HIERTCN_OK;
 }
 
-#define ROWS_GO(kernel, blocks, ...)                                                                                                           \
+#define ROWS_VEC(kernel, dt, wide, tpr, g, ...)                                                                                                \
   do {                                                                                                                                         \
-    const dim3 g_((unsigned)(blocks)), b_(NT);                                                                                                 \
-    if (p.a.dtype == HIERTCN_FP32 && vec == 1) hipLaunchKernelGGL((kernel<HIERTCN_FP32, 1>), g_, b_, 0, st, __VA_ARGS__);                       \
-    else if (p.a.dtype == HIERTCN_FP32) hipLaunchKernelGGL((kernel<HIERTCN_FP32, 4>), g_, b_, 0, st, __VA_ARGS__);                              \
-    else if (p.a.dtype == HIERTCN_BF16 && vec == 1) hipLaunchKernelGGL((kernel<HIERTCN_BF16, 1>), g_, b_, 0, st, __VA_ARGS__);                  \
-    else if (p.a.dtype == HIERTCN_BF16) hipLaunchKernelGGL((kernel<HIERTCN_BF16, 8>), g_, b_, 0, st, __VA_ARGS__);                              \
-    else if (vec == 1) hipLaunchKernelGGL((kernel<HIERTCN_FP16, 1>), g_, b_, 0, st, __VA_ARGS__);                                               \
-    else hipLaunchKernelGGL((kernel<HIERTCN_FP16, 8>), g_, b_, 0, st, __VA_ARGS__);                                                             \
-    OPS_TRY(hipGetLastError());                                                                                                                 \
+    if (vec == 1 && tpr == NT) hipLaunchKernelGGL((kernel<dt, 1, NT>), g, dim3(NT), 0, st, __VA_ARGS__);                                        \
+    else if (vec == 1) hipLaunchKernelGGL((kernel<dt, 1, 64>), g, dim3(NT), 0, st, __VA_ARGS__);                                                \
+    else if (tpr == NT) hipLaunchKernelGGL((kernel<dt, wide, NT>), g, dim3(NT), 0, st, __VA_ARGS__);                                            \
+    else hipLaunchKernelGGL((kernel<dt, wide, 64>), g, dim3(NT), 0, st, __VA_ARGS__);                                                           \
+  } while (0)
+#define ROWS_GO(kernel, cut, extra, ...)                                                                                                       \
+  do {                                                                                                                                         \
+    const dim3 g_((unsigned)(workgroups(cut, p.R) + (extra)));                                                                                 \
+    if (p.a.dtype == HIERTCN_FP32) ROWS_VEC(kernel, HIERTCN_FP32, 4, cut.tpr, g_, __VA_ARGS__);                                                 \
+    else if (p.a.dtype == HIERTCN_BF16) ROWS_VEC(kernel, HIERTCN_BF16, 8, cut.tpr, g_, __VA_ARGS__);                                            \
+    else ROWS_VEC(kernel, HIERTCN_FP16, 8, cut.tpr, g_, __VA_ARGS__);                                                                           \
+    OPS_TRY(hipGetLastError());                                                                                                                \
   } while (0)
 
 int check_out(const RowsP& p, const void* q, int64_t n, const char* name) {
@@ -424,7 +552,7 @@ int check_out(const RowsP& p, const void* q, int64_t n, const char* name) {
 
 int finish(const RowsP& p, int vec, const Sums& s, hipStream_t st) {
   if (p.a.dlogits) {
-    ROWS_GO(k_dlogits, p.R * p.parts + 1, p, s);
+    ROWS_GO(k_dlogits, p.write, 1, p, s);
   } else {
     hipLaunchKernelGGL(k_sums, dim3(1), dim3(NT), 0, st, s);
     OPS_TRY(hipGetLastError());
@@ -445,8 +573,8 @@ int hiertcn_sequence_logp(const hiertcn_rows_t* r, void* stream) {
   int vec;
   if (int rc = prepare(r, false, p, vec)) return rc;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  ROWS_GO(k_part, p.R * p.parts, p);
-  hipLaunchKernelGGL(k_logp, dim3((unsigned)((p.R + NT - 1) / NT)), dim3(NT), 0, st, p);
+  ROWS_GO(k_part, p.read, 0, p);
+  hipLaunchKernelGGL(k_logp, dim3((unsigned)p.groups), dim3(NT), 0, st, p);
   OPS_TRY(hipGetLastError());
   return HIERTCN_OK;
 }
@@ -471,10 +599,10 @@ int hiertcn_preference_loss(const hiertcn_rows_t* r, const hiertcn_preference_t*
       if (ops_overlap(ops_flat(outs[i].q, outs[i].n, 4), ops_flat(outs[j].q, outs[j].n, 4))) return ops_fail(HIERTCN_ERR_INVALID, "%s overlaps %s", outs[i].name, outs[j].name);
   }
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  ROWS_GO(k_part, p.R * p.parts, p);
-  hipLaunchKernelGGL(k_pairs, dim3((unsigned)P), dim3(NT), 0, st, p, *q);
+  ROWS_GO(k_part, p.read, 0, p);
+  hipLaunchKernelGGL(k_pairs, dim3((unsigned)P), dim3(PAIR_NT), 0, st, p, *q);
   OPS_TRY(hipGetLastError());
-  return finish(p, vec, Sums{q->pair_loss, P, 1.f / (float)P, {q->loss, nullptr, nullptr}}, st);
+  return finish(p, vec, Sums{q->pair_loss, nullptr, P, 1.0 / (double)P, {q->loss, nullptr, nullptr}}, st);
 }
 
 int hiertcn_policy_loss(const hiertcn_rows_t* r, const hiertcn_policy_t* q, void* stream) {
@@ -505,10 +633,11 @@ int hiertcn_policy_loss(const hiertcn_rows_t* r, const hiertcn_policy_t* q, void
   for (const OpsView& v : ins)
     if (ops_overlap(lp, v) || ops_overlap(d, v) || ops_overlap(ws, v)) return ops_fail(HIERTCN_ERR_INVALID, "logp, dlogits or the workspace overlaps an input");
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  ROWS_GO(k_part, p.R * p.parts + a.n, p);
-  hipLaunchKernelGGL(k_policy, dim3((unsigned)((p.R + NT - 1) / NT)), dim3(NT), 0, st, p, *q);
+  p.counters = counters_of(a.n, a.T);
+  ROWS_GO(k_part, p.read, p.counters, p);
+  hipLaunchKernelGGL(k_policy, dim3((unsigned)p.groups), dim3(NT), 0, st, p, *q);
   OPS_TRY(hipGetLastError());
-  return finish(p, vec, Sums{p.term, p.R, 1.f, {q->loss, q->kl, q->clipped}}, st);
+  return finish(p, vec, Sums{nullptr, p.term, p.groups, 1.0, {q->loss, q->kl, q->clipped}}, st);
 }
 
 }  // extern "C"

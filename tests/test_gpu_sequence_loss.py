@@ -65,9 +65,12 @@ def test_preference(shape, dtype):
     for k in ("loss", "pair_loss", "margin", "seq_logp", "logp"):
         close(out[k], want, k)
     close(out["dlogits"], want, "dlogits", dtype)
-    assert torch.equal(sequence_logp(z, ids), out["logp"])
+    # without a gradient a row is summed in other parts: the same bounds, not the same bits
+    close(sequence_logp(z, ids), want, "logp")
     less = preference_loss(z, ids, ref, beta=0.3, kind=kind, label_smoothing=smoothing, average=shape[1] % 2 == 0, want_grad=False)
-    assert less["dlogits"] is None and torch.equal(less["loss"], out["loss"])
+    assert less["dlogits"] is None
+    for k in ("loss", "pair_loss", "margin", "seq_logp", "logp"):
+        close(less[k], want, k)
     again = preference_loss(z, ids, ref, beta=0.3, kind=kind, label_smoothing=smoothing, average=shape[1] % 2 == 0, grad_scale=scale, dlogits=z)
     assert again["dlogits"] is z and torch.equal(z, out["dlogits"])
 
@@ -100,7 +103,8 @@ def test_policy(shape, dtype, mean):
         close(out[k], want, k)
     close(out["dlogits"], want, "dlogits", dtype)
     less = policy_loss(z, ids, old, adv, ref_logp=ref if with_ref else None, clip_low=0.2, clip_high=0.28, kl_coef=0.05 if with_ref else 0.0, mean=mean, want_grad=False)
-    assert all(torch.equal(less[k], out[k]) for k in ("loss", "kl", "clipped", "logp"))
+    for k in ("loss", "kl", "clipped", "logp"):
+        close(less[k], want, k)
     policy_loss(z, ids, old, adv, ref_logp=ref if with_ref else None, clip_low=0.2, clip_high=0.28, kl_coef=0.05 if with_ref else 0.0, mean=mean, grad_scale=scale, dlogits=z)
     assert torch.equal(z, out["dlogits"])
 
