@@ -31,33 +31,34 @@ struct Batch {
 };
 static_assert(sizeof(Batch) <= 4096, "kernel arguments");
 
-__device__ __forceinline__ uint32_t mix(uint64_t e, uint32_t key) {
-  uint32_t x = (uint32_t)e * 0x9E3779B1u + key + (uint32_t)(e >> 32) * 0x1F83D9ABu;
+// random bits of element e.  (Its high word is a block's: blocks of 256 do not cross 2^32.)
+__device__ __forceinline__ uint32_t mix(uint32_t e, uint32_t key) {
+  uint32_t x = e * 0x9E3779B1u + key;
   x = (x ^ (x >> 16)) * 0x3C6EF373u;
   x = (x ^ (x >> 15)) * 0x510E527Fu;
   return x ^ (x >> 16);
 }
 
-// where a lane's four elements of a block lie: neighbours where the addresses allow it, else 64 apart
+// where a lane's four elements of a block lie: neighbours where the addresses allow it, else 64 apart.  FULL: known to be all there, side by side
+template <bool FULL>
 struct Lane {
   int64_t base;
   int step, n;                           // element i: base + i * step; the first n exist
+  __device__ __forceinline__ Lane(int64_t block, int64_t numel, bool wide) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (FULL) wide = true;
+    step = wide ? 1 : 64;
+    base = block * BLOCK + (wide ? lane * 4 : lane);
+    const int64_t left = numel - base;
+    n = FULL ? 4 : left <= 0 ? 0 : wide ? (left < 4 ? (int)left : 4) : (int)((left + 63) / 64 < 4 ? (left + 63) / 64 : 4);
+  }
 };
-__device__ __forceinline__ Lane lane_of(int64_t block, int64_t numel, bool wide) {
-  const int lane = threadIdx.x & 63;
-  Lane l;
-  l.step = wide ? 1 : 64;
-  l.base = block * BLOCK + (wide ? lane * 4 : lane);
-  const int64_t left = numel - l.base;
-  l.n = left <= 0 ? 0 : wide ? (left < 4 ? (int)left : 4) : (int)((left + 63) / 64 < 4 ? (left + 63) / 64 : 4);
-  return l;
-}
 template <typename T>
 struct alignas(4 * sizeof(T)) Four { T v[4]; };
-template <typename T>
-__device__ __forceinline__ void load4(const void* p, const Lane& l, T (&o)[4]) {
+template <typename T, bool FULL>
+__device__ __forceinline__ void load4(const void* p, const Lane<FULL>& l, T (&o)[4]) {
   const T* q = static_cast<const T*>(p) + l.base;
-  if (l.step == 1 && l.n == 4) {
+  if (FULL || (l.step == 1 && l.n == 4)) {
     const Four<T> x = *reinterpret_cast<const Four<T>*>(q);
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] = x.v[i];
@@ -66,21 +67,22 @@ __device__ __forceinline__ void load4(const void* p, const Lane& l, T (&o)[4]) {
     for (int i = 0; i < 4; i++) o[i] = i < l.n ? q[i * l.step] : T(0);
   }
 }
-template <typename T>
-__device__ __forceinline__ void store4(void* p, const Lane& l, const T (&o)[4]) {
+template <typename T, bool FULL>
+__device__ __forceinline__ void store4(void* p, const Lane<FULL>& l, const T (&o)[4]) {
   T* q = static_cast<T*>(p) + l.base;
-  if (l.step == 1 && l.n == 4) {
+  if (FULL || (l.step == 1 && l.n == 4)) {
     Four<T> x;
 #pragma unroll
     for (int i = 0; i < 4; i++) x.v[i] = o[i];
-    *reinterpret_cast<Four<T>*>(q) = x;
+    ops_put<true>(q, x);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; i++)
       if (i < l.n) q[i * l.step] = o[i];
   }
 }
-__device__ __forceinline__ void load_grad(const hiertcn_adamw_tensor_t& t, const Lane& l, float (&g)[4]) {
+template <bool FULL>
+__device__ __forceinline__ void load_grad(const hiertcn_adamw_tensor_t& t, const Lane<FULL>& l, float (&g)[4]) {
   if (t.grad_dtype == HIERTCN_FP32) {
     load4<float>(t.grad, l, g);
   } else {
@@ -90,14 +92,24 @@ __device__ __forceinline__ void load_grad(const hiertcn_adamw_tensor_t& t, const
     for (int i = 0; i < 4; i++) g[i] = t.grad_dtype == HIERTCN_BF16 ? ops_h2f(h[i], HIERTCN_BF16) : ops_h2f(h[i], HIERTCN_FP16);
   }
 }
-__device__ __forceinline__ float wave_max(float x) {      // NaN wins
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const float y = __shfl_xor(x, d);
-    x = y > x || y != y ? y : x;
-  }
-  return x;
+__device__ __forceinline__ float lane_of(float x, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane)); }
+// the largest of the wave's magnitudes, as bits: unsigned numbers in the order of the floats they hold, NaNs above them all.  Steps of 1, 2, 4, 8 lanes inside rows
+// of 16, then a row into the next and a half into the next; the last lane has it.
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_of(uint32_t x) {
+  const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, false);
+  return x > y ? x : y;
 }
+__device__ __forceinline__ float wave_max(uint32_t x) {
+  x = max_of<0x111>(x);
+  x = max_of<0x112>(x);
+  x = max_of<0x114>(x);
+  x = max_of<0x118>(x);
+  x = max_of<0x142>(x);
+  x = max_of<0x143>(x);
+  return lane_of(__builtin_bit_cast(float, x), 63);
+}
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
 __device__ __forceinline__ float decode_m(int q, float scale) {
 #pragma clang fp contract(off)
   const float f = (float)q * (1.f / 127.f);
@@ -109,13 +121,36 @@ __device__ __forceinline__ float decode_v(uint32_t q, float scale) {
   const float x = f * f * scale;
   return x * x;
 }
+// sqrt(v), rounded: the hardware's reciprocal root and one correction, which is the rounded root for every mantissa of both binades (all 2^24 were compared) as
+// long as neither v nor the correction leaves the normal range; the library's root for zero, tiny, huge and what is no number.  Half its operations.
+__device__ __forceinline__ float root_of(float v) {
+  const float y = __builtin_amdgcn_rsqf(v), x = v * y;
+  float s = __builtin_fmaf(__builtin_fmaf(-x, x, v), 0.5f * y, x);
+  if (__builtin_expect(__builtin_bit_cast(uint32_t, v) - 0x0d800000u >= 0x65000000u, 0)) {      // outside of 2^-100 .. 2^102
+    asm volatile("");
+    s = sqrtf(v);
+  }
+  return s;
+}
+// n / d to within a unit of its last place; zeros, infinities and NaNs as a division has them
+__device__ __forceinline__ float quotient(float n, float d) {
+  const float y = __builtin_amdgcn_rcpf(d), q = n * y;
+  return __builtin_amdgcn_div_fixupf(__builtin_fmaf(__builtin_fmaf(-d, q, n), y, q), d, n);
+}
 // code of a magnitude: the largest a with a <= r, or the next one up with the probability that keeps the expectation
 template <bool SQUARED>
 __device__ __forceinline__ int encode(float mag, float inv, uint32_t bits) {
 #pragma clang fp contract(off)
   constexpr float TOP = SQUARED ? 255.f : 127.f;
   float r = mag * inv;
-  const float q = fminf(floorf(sqrtf(r) * TOP), TOP - 1.f);
+  // q = floor(sqrt(r) TOP), at most TOP - 1.  The hardware's root is off by a unit of its last place, which matters only next to a whole number: there the
+  // rounded root is taken (a lane in 2000; the empty asm keeps the compiler from taking it for all).  Cut to [1/2, TOP - 1/2] the ends are not such a place.
+  float y = __builtin_amdgcn_fmed3f(__builtin_amdgcn_sqrtf(r) * TOP, 0.5f, TOP - 0.5f);
+  if (__builtin_expect(fabsf(__builtin_amdgcn_fractf(y) - 0.5f) > 0.499755859375f, 0)) {
+    asm volatile("");
+    y = __builtin_amdgcn_fmed3f(sqrtf(r) * TOP, 0.5f, TOP - 0.5f);
+  }
+  const float q = floorf(y);
   float a = q * (1.f / TOP), b = (q + 1.f) * (1.f / TOP);
   a = a * a;
   b = b * b;
@@ -125,49 +160,48 @@ __device__ __forceinline__ int encode(float mag, float inv, uint32_t bits) {
     r = r * r;
   }
   const float u = (float)bits * 1.52587890625e-5f;
-  const int code = (int)fmaxf(q, 0.f) + (r - a > u * (b - a) ? 1 : 0);
+  const int code = (int)q + (r - a > u * (b - a) ? 1 : 0);
   return SQUARED && mag > 0.f && inv > 0.f && code < 1 ? 1 : code;
 }
 __device__ __forceinline__ float scale_of(float largest) { return largest < 7.888609052210118e-31f ? 0.f : largest; }      // 2^-100
 __device__ __forceinline__ float inverse_of(float scale) { return scale > 0.f ? 1.f / scale : 0.f; }
 
-__device__ __forceinline__ int tensor_of(const Batch& b, uint32_t wg) {
+template <typename B>
+__device__ __forceinline__ int tensor_of(const B& b, uint32_t wg) {
   int i = 0;
   while (i + 1 < b.n && wg >= b.first[i + 1]) i++;
   return i;
 }
 
-template <bool Q8>
-__global__ __launch_bounds__(NT) void k_adamw(Batch b) {
+template <bool Q8, bool FULL>
+__device__ __forceinline__ void update(const Batch& b, const hiertcn_adamw_tensor_t& t, int64_t block, bool wide, float decay) {
 #pragma clang fp contract(off)
-  const int i = tensor_of(b, blockIdx.x);
-  const hiertcn_adamw_tensor_t& t = b.t[i];
-  const int64_t block = (int64_t)(blockIdx.x - b.first[i]) * PER_WG + (threadIdx.x >> 6);
-  if (block * BLOCK >= t.numel) return;
-  const Lane l = lane_of(block, t.numel, b.wide >> i & 1);
+  const Lane<FULL> l(block, t.numel, wide);
   const float gs = b.gscale_dev ? b.gscale * b.gscale_dev[0] : b.gscale;
   float p[4], g[4], m[4], v[4], s[4];
-  load4<float>(t.param, l, p);
-  load_grad(t, l, g);
   if constexpr (Q8) {
     int8_t qm[4];
     uint8_t qv[4];
     load4<int8_t>(t.m, l, qm);
     load4<uint8_t>(t.v, l, qv);
     const float sm = t.m_scale[block], sv = t.v_scale[block];
+    load4<float>(t.param, l, p);
+    load_grad(t, l, g);
 #pragma unroll
     for (int k = 0; k < 4; k++) m[k] = decode_m(qm[k], sm), v[k] = decode_v(qv[k], sv);
   } else {
     load4<float>(t.m, l, m);
     load4<float>(t.v, l, v);
+    load4<float>(t.param, l, p);
+    load_grad(t, l, g);
   }
 #pragma unroll
   for (int k = 0; k < 4; k++) {
     const float gk = g[k] * gs;
     m[k] = m[k] * b.b1 + gk * b.c1;
     v[k] = v[k] * b.b2 + gk * gk * b.c2;
-    s[k] = sqrtf(v[k]);
-    p[k] = p[k] * b.decay[i] - b.step * (m[k] / (s[k] * b.root + b.eps));
+    s[k] = root_of(v[k]);
+    p[k] = p[k] * decay - b.step * quotient(m[k], s[k] * b.root + b.eps);
   }
   store4<float>(t.param, l, p);
   if (t.copy) {
@@ -177,22 +211,22 @@ __global__ __launch_bounds__(NT) void k_adamw(Batch b) {
     store4<uint16_t>(t.copy, l, h);
   }
   if constexpr (Q8) {
-    float tm = 0.f, tv = 0.f;
+    uint32_t tm = 0, tv = 0;
 #pragma unroll
     for (int k = 0; k < 4; k++)
       if (k < l.n) {
-        const float am = fabsf(m[k]);
-        tm = am > tm || am != am ? am : tm;
-        tv = s[k] > tv || s[k] != s[k] ? s[k] : tv;
+        tm = tm > magnitude(m[k]) ? tm : magnitude(m[k]);
+        tv = tv > magnitude(s[k]) ? tv : magnitude(s[k]);
       }
     const float sm = scale_of(wave_max(tm)), sv = scale_of(wave_max(tv));
-    const float im = inverse_of(sm), iv = inverse_of(sv);
+    const float inv = inverse_of(threadIdx.x & 1 ? sv : sm);                                    // one division for both
+    const float im = lane_of(inv, 0), iv = lane_of(inv, 1);
     int8_t qm[4];
     uint8_t qv[4];
-    const uint32_t key = b.key + (uint32_t)t.index * 0xBB67AE85u;
+    const uint32_t key = b.key + (uint32_t)t.index * 0xBB67AE85u + (uint32_t)((uint64_t)(block * BLOCK) >> 32) * 0x1F83D9ABu;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      const uint32_t bits = mix((uint64_t)(l.base + k * l.step), key);
+      const uint32_t bits = mix((uint32_t)(l.base + k * l.step), key);
       const int c = encode<false>(fabsf(m[k]), im, bits & 0xffffu);
       qm[k] = (int8_t)(m[k] < 0.f ? -c : c);
       qv[k] = (uint8_t)encode<true>(s[k], iv, bits >> 16);
@@ -206,6 +240,22 @@ __global__ __launch_bounds__(NT) void k_adamw(Batch b) {
   }
 }
 
+// the wave's first block of its tensor, of EACH.  false: behind its end
+template <int EACH, typename B>
+__device__ __forceinline__ bool block_here(const B& b, int i, int64_t& block) {
+  block = ((int64_t)(blockIdx.x - b.first[i]) * PER_WG + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * EACH;
+  return block * BLOCK < b.t[i].numel;
+}
+template <bool Q8>
+__global__ __launch_bounds__(NT) void k_adamw(Batch b) {
+  const int i = tensor_of(b, blockIdx.x);
+  int64_t block;
+  if (!block_here<1>(b, i, block)) return;
+  const bool wide = b.wide >> i & 1;
+  if (wide && (block + 1) * BLOCK <= b.t[i].numel) update<Q8, true>(b, b.t[i], block, wide, b.decay[i]);
+  else update<Q8, false>(b, b.t[i], block, wide, b.decay[i]);
+}
+
 struct DecodeBatch {
   struct { int64_t numel; const void* m; const void* v; const float* ms; const float* vs; float* mo; float* vo; } t[MAX_TENSORS];
   uint32_t first[MAX_TENSORS + 1];
@@ -213,30 +263,42 @@ struct DecodeBatch {
   uint64_t wide;
 };
 static_assert(sizeof(DecodeBatch) <= 4096, "kernel arguments");
+// a wave decodes WAVE_BLOCKS blocks of a tensor, all loads first
+constexpr int WAVE_BLOCKS = 4;
+template <bool FULL, typename T>
+__device__ __forceinline__ void decode_blocks(const T& t, int64_t block, bool wide) {
+  int8_t qm[WAVE_BLOCKS][4];
+  uint8_t qv[WAVE_BLOCKS][4];
+  float sm[WAVE_BLOCKS], sv[WAVE_BLOCKS], o[4];
+#pragma unroll
+  for (int j = 0; j < WAVE_BLOCKS; j++) {
+    const Lane<FULL> l(block + j, t.numel, wide);
+    const bool here = FULL || (block + j) * BLOCK < t.numel;
+    if (t.mo) load4<int8_t>(t.m, l, qm[j]), sm[j] = here ? t.ms[block + j] : 0.f;
+    if (t.vo) load4<uint8_t>(t.v, l, qv[j]), sv[j] = here ? t.vs[block + j] : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < WAVE_BLOCKS; j++) {
+    const Lane<FULL> l(block + j, t.numel, wide);
+    if (t.mo) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) o[k] = decode_m(qm[j][k], sm[j]);
+      store4<float>(t.mo, l, o);
+    }
+    if (t.vo) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) o[k] = decode_v(qv[j][k], sv[j]);
+      store4<float>(t.vo, l, o);
+    }
+  }
+}
 __global__ __launch_bounds__(NT) void k_moments(DecodeBatch b) {
-  int i = 0;
-  while (i + 1 < b.n && blockIdx.x >= b.first[i + 1]) i++;
-  const auto& t = b.t[i];
-  const int64_t block = (int64_t)(blockIdx.x - b.first[i]) * PER_WG + (threadIdx.x >> 6);
-  if (block * BLOCK >= t.numel) return;
-  const Lane l = lane_of(block, t.numel, b.wide >> i & 1);
-  float o[4];
-  if (t.mo) {
-    int8_t q[4];
-    load4<int8_t>(t.m, l, q);
-    const float s = t.ms[block];
-#pragma unroll
-    for (int k = 0; k < 4; k++) o[k] = decode_m(q[k], s);
-    store4<float>(t.mo, l, o);
-  }
-  if (t.vo) {
-    uint8_t q[4];
-    load4<uint8_t>(t.v, l, q);
-    const float s = t.vs[block];
-#pragma unroll
-    for (int k = 0; k < 4; k++) o[k] = decode_v(q[k], s);
-    store4<float>(t.vo, l, o);
-  }
+  const int i = tensor_of(b, blockIdx.x);
+  int64_t block;
+  if (!block_here<WAVE_BLOCKS>(b, i, block)) return;
+  const bool wide = b.wide >> i & 1;
+  if (wide && (block + WAVE_BLOCKS) * BLOCK <= b.t[i].numel) decode_blocks<true>(b.t[i], block, wide);
+  else decode_blocks<false>(b.t[i], block, wide);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------------------------
@@ -342,7 +404,7 @@ int hiertcn_adamw_moments(const hiertcn_adamw_tensor_t* tensors, int64_t n, floa
     for (; i < n && b.n < MAX_TENSORS; i++) {
       const hiertcn_adamw_tensor_t& t = tensors[i];
       if (t.numel == 0 || (!m_out[i] && !v_out[i])) continue;
-      const uint64_t blocks = (uint64_t)(t.numel + BLOCK - 1) / BLOCK, w = (blocks + PER_WG - 1) / PER_WG;
+      const uint64_t blocks = (uint64_t)(t.numel + BLOCK - 1) / BLOCK, w = (blocks + PER_WG * WAVE_BLOCKS - 1) / (PER_WG * WAVE_BLOCKS);
       if (w > 0x7fffffffull) return ops_fail(HIERTCN_ERR_INVALID, "tensor %lld: too large for one launch", (long long)i);
       if (wgs + w > 0x7fffffffull) break;
       b.t[b.n] = {t.numel, t.m, t.v, t.m_scale, t.v_scale, m_out[i], v_out[i]};
