@@ -35,20 +35,20 @@ class AdamW:
         self.device = _ops.on_gpu(self.params[0], "params[0]")
         for i, p in enumerate(self.params):
             need(p, f"params[{i}]", torch.float32, self.device, p.shape if isinstance(p, torch.Tensor) else ())
-        decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
         copies = [None] * n if copies is None else list(copies)
-        if len(decay) != n or len(copies) != n:
-            raise HierTCNError(f"{n} parameters, {len(decay)} weight decays, {len(copies)} copies")
+        if len(copies) != n:
+            raise HierTCNError(f"{n} parameters, {len(copies)} copies")
         self.lr, self.betas, self.eps, self.state_bits, self.seed, self.t = float(lr), (float(betas[0]), float(betas[1])), float(eps), state_bits, int(seed), 0
-        self.weight_decay, self.copies = decay, copies
+        self.copies = copies
         self._desc = (_ops.AdamwTensor * n)()
         self._flat = [torch.Size([p.numel()]) for p in self.params]
         for i, (p, c, d) in enumerate(zip(self.params, copies, self._desc)):
-            d.numel, d.param, d.weight_decay, d.index = p.numel(), p.data_ptr(), decay[i], i
+            d.numel, d.param, d.index = p.numel(), p.data_ptr(), i
             if c is not None:
                 if not isinstance(c, torch.Tensor) or c.dtype not in (torch.bfloat16, torch.float16):
                     raise HierTCNError(f"copies[{i}]: a bfloat16 or float16 tensor")
                 d.copy, d.copy_dtype = need(c, f"copies[{i}]", c.dtype, self.device, p.shape).data_ptr(), _ops.DTYPE[c.dtype]
+        self.set_weight_decay(weight_decay)
         zeros = lambda dt, block=1: [torch.zeros(-(-p.numel() // block), dtype=dt, device=self.device) for p in self.params]  # noqa: E731
         if state_bits == 32:
             self._attach(zeros(torch.float32), zeros(torch.float32), None, None)
@@ -58,6 +58,16 @@ class AdamW:
         if grads is not None:
             self._bind(grads)
             self.grads = list(grads)
+
+    def set_weight_decay(self, weight_decay: Union[float, Sequence[float]]):
+        """One value, or one per tensor, from the next step on."""
+        n = len(self.params)
+        decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+        if len(decay) != n:
+            raise HierTCNError(f"{n} parameters, {len(decay)} weight decays")
+        for d, w in zip(self._desc, decay):
+            d.weight_decay = w
+        self.weight_decay = decay
 
     def _attach(self, m, v, m_scale, v_scale):
         dm, dv = (torch.float32, torch.float32) if self.state_bits == 32 else (torch.int8, torch.uint8)

@@ -9,11 +9,13 @@ Mirrors /root/reference/args.py:3-206 (flags and defaults), :208-228 (input path
   * `--emb_dim` is added: the reference hard-codes 128 for the item-embedding / projection width
     (model_hier.py:50,85; model_tcn.py:35); BASELINE.json's configs vary it ("d");
   * `--storage_dtype` is added: bf16 (production), fp16 or fp32 -- the exact evaluation mode that
-    computes everything in fp32 like the reference's graph (for parity runs on trained checkpoints).
+    computes everything in fp32 like the reference's graph (for parity runs on trained checkpoints);
+  * `--optimizer adamw` and `--weight_decay` are added: Adam with decoupled weight decay in place of model.py:139's Adam.  They are attributes of the
+    Namespace only where they are given.
 """
 from __future__ import annotations
 
-from argparse import ArgumentParser, Namespace
+from argparse import SUPPRESS, ArgumentParser, Namespace
 
 
 def _int_list(s):
@@ -103,6 +105,8 @@ def build_parser() -> ArgumentParser:
     p.add_argument("--test_data_ratio", dest="test_data_ratio", default=1, type=float)
     p.add_argument("--data_splits", dest="data_splits", default=100, type=int)
     # build-only addition (see module docstring)
+    p.add_argument("--optimizer", dest="optimizer", default=SUPPRESS, choices=["adam", "adamw"])
+    p.add_argument("--weight_decay", dest="weight_decay", default=SUPPRESS, type=float)
     p.add_argument("--emb_dim", dest="emb_dim", default=128, type=int)
     p.add_argument("--storage_dtype", dest="storage_dtype", default="bf16", choices=["bf16", "fp16", "fp32", "split16"])
     # args.py:193 -- the "eval" default set

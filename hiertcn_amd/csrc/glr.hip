@@ -595,7 +595,8 @@ int glr(const hiertcn_glr_t* in, bool backward, hipStream_t st) {
     p.state0 = reinterpret_cast<float*>(p.map + words_of(q, a.B, a.D));
     p.ticket = reinterpret_cast<unsigned*>(p.state0 + (a.B * a.D + 31) / 32 * 32);
   }
-  OPS_TRY(a.dtype == HIERTCN_FP32 ? go_vec<HIERTCN_FP32>(p, q, backward, st) : a.dtype == HIERTCN_BF16 ? go_vec<HIERTCN_BF16>(p, q, backward, st) : go_vec<HIERTCN_FP16>(p, q, backward, st));
+  const hipError_t launched = a.dtype == HIERTCN_FP32 ? go_vec<HIERTCN_FP32>(p, q, backward, st) : a.dtype == HIERTCN_BF16 ? go_vec<HIERTCN_BF16>(p, q, backward, st) : go_vec<HIERTCN_FP16>(p, q, backward, st);
+  OPS_TRY(launched);
   return HIERTCN_OK;
 }
 

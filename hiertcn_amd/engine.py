@@ -44,7 +44,7 @@ def _req(t: torch.Tensor, dtype, name: str, shape=None):
 UNSUPPORTED_FLAGS = ("has_gap", "has_impression", "has_batchnorm", "has_weightnorm", "has_layernorm", "l2_normalize")
 
 
-def check_supported(args, train: bool = False, loss_ok=("cross_entropy",)):
+def check_supported(args, train: bool = False, loss_ok=("cross_entropy",), optimizer_ok=("adam", "adamw")):
     """The ONE place that refuses model-changing flags the hot path does not implement.  Every entry
     point builds an Engine, and Engine() builds its config here, so neither the model_hier / model_tcn shims nor the run loops
     nor the CLI can accept such a flag and silently run something else under the requested run name (args.py:232-240)."""
@@ -55,6 +55,10 @@ def check_supported(args, train: bool = False, loss_ok=("cross_entropy",)):
         raise NotImplementedError("args.data_noise is outside the hot path")
     if getattr(args, "loss", "cross_entropy") not in loss_ok:
         raise NotImplementedError(f"args.loss={args.loss!r}: this model is built for {loss_ok} (loss.py:20-21, 247-257)")
+    if getattr(args, "optimizer", "adam") not in optimizer_ok:
+        raise NotImplementedError(f"args.optimizer={args.optimizer!r}: this model trains with {' or '.join(optimizer_ok)}")
+    if float(getattr(args, "weight_decay", 0.0)) != 0.0 and getattr(args, "optimizer", "adam") != "adamw":
+        raise NotImplementedError("args.weight_decay belongs to args.optimizer = 'adamw' (model.py:139's Adam has none)")
     if train and float(getattr(args, "dropout", 0.0) or 0.0) != 0.0:
         raise NotImplementedError("args.dropout != 0 while training: tf.layers.Dropout after conv1 (customized_tcn_cell.py:119) "
                                   "is not built; the reference default is 0.0")
@@ -131,6 +135,8 @@ class Engine:
             if self.exact:   # allocates the weight copies of the mode, which set_weights fills; must precede set_weights
                 self._ck(self.lib.hiertcn_set_precision(self._h, _lib.PRECISION_SPLIT16 if self.mode == "split16" else _lib.PRECISION_FP32))
         self.train = bool(train)
+        self.optimizer, self.weight_decay = getattr(args, "optimizer", "adam"), float(getattr(args, "weight_decay", 0.0))
+        self._adamw = None
         if self.train:   # fp32 masters / gradients / Adam moments; must precede set_weights
             with torch.cuda.device(self.device):
                 self._ck(self.lib.hiertcn_train_enable(self._h))
@@ -177,7 +183,7 @@ class Engine:
     def close(self):
         if getattr(self, "_h", None) is not None and self._h.value:
             self.lib.hiertcn_destroy(self._h)
-            self._h = C.c_void_p()
+            self._h, self._adamw = C.c_void_p(), None
             _LIVE_ENGINES.discard(self)
 
     def __del__(self):  # pragma: no cover
@@ -577,6 +583,31 @@ class Engine:
     def adam_step(self, lr: float, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, grad_scale: float = 1.0):
         """tf.train.AdamOptimizer(lr) defaults (model.py:139)."""
         self._ck(self.lib.hiertcn_adam_step(self._h, float(lr), float(beta1), float(beta2), float(eps), float(grad_scale), self._stream()))
+
+    def adamw_step(self, lr: float, weight_decay: float = 0.0, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, grad_scale: float = 1.0):
+        """Adam with decoupled weight decay (adamw.AdamW) in place of adam_step: theta <- (1 - lr * weight_decay) theta - lr m^ / (sqrt(v^) + eps), the decay on
+        every variable.  The moments are the handle's own (optimizer_state / load_optimizer_state and the time step serve both), in fp32."""
+        if self._adamw is None:
+            from . import _ops
+            from .adamw import AdamW
+            _ops.bind(self.lib)
+            self._adamw = AdamW([self._arena(0)], [self._arena(1)])
+        opt, t = self._adamw, C.c_int64(0)
+        self._ck(self.lib.hiertcn_adam_time(self._h, C.byref(t), None))
+        opt.betas, opt.eps = (float(beta1), float(beta2)), float(eps)
+        opt.set_weight_decay(weight_decay)
+        opt.set_state([self._arena(2)], [self._arena(3)], t.value)
+        opt.step(lr=lr, grad_scale=grad_scale)
+        t.value += 1
+        self._ck(self.lib.hiertcn_adam_time(self._h, None, C.byref(t)))
+        self._ck(self.lib.hiertcn_train_masters_changed(self._h, self._stream()))
+
+    def optimizer_step(self, lr: float, grad_scale: float = 1.0):
+        """The step that args.optimizer names: 'adam' (the default, model.py:139) or 'adamw' with args.weight_decay."""
+        if self.optimizer == "adamw":
+            self.adamw_step(lr, weight_decay=self.weight_decay, grad_scale=grad_scale)
+        else:
+            self.adam_step(lr, grad_scale=grad_scale)
 
     def export(self, which: str = "weights", root: Optional[str] = None) -> Dict[str, np.ndarray]:
         """Masters ('weights') or gradients ('grads') as {TF variable name: fp32 ndarray in the reference layout}."""

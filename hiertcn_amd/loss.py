@@ -9,7 +9,8 @@ from __future__ import annotations
 
 import torch
 
-from .model import LazyLogits
+from . import sequence_loss
+from .model import LazyLogits, _to_ids
 
 
 def _need_lazy(pred):
@@ -25,6 +26,36 @@ def calc_loss(pred, y, y_impression=None, loss="cross_entropy"):
     if loss != "cross_entropy" or y_impression is not None:
         raise NotImplementedError("only the cross_entropy loss of the XING path is built")
     return pred.unpad(pred.scored(y)["ce"])
+
+
+def _answers(pred, y):
+    _need_lazy(pred)
+    logits = pred.materialize()
+    return logits, torch.as_tensor(_to_ids(y), device=logits.device).to(torch.int32).contiguous()
+
+
+def calc_sequence_logp(pred, y):
+    """Log-probability of every answer y [B, T] (0 where there is none) -> [B, T] fp32: what the two losses below want of a reference model and of the policy
+    that chose the answers.  The logits are materialised (4 N bytes a step)."""
+    return sequence_loss.sequence_logp(*_answers(pred, y))
+
+
+def calc_preference(pred, y, ref_logp, **options):
+    """sequence_loss.preference_loss on a model's pred: lanes 0 .. B/2-1 are the preferred sequences, lanes B/2 .. B-1 their counterparts, ref_logp [B] the
+    reference model's sums.  options: beta, kind, label_smoothing, average, grad_scale, want_grad.  The gradient takes the place of the logits."""
+    logits, ids = _answers(pred, y)
+    if options.get("want_grad", True):
+        options.setdefault("dlogits", logits)
+    return sequence_loss.preference_loss(logits, ids, ref_logp, **options)
+
+
+def calc_policy(pred, y, old_logp, advantage, **options):
+    """sequence_loss.policy_loss on a model's pred: old_logp [B, T], advantage [B] or [B, T].  options: ref_logp, clip_low, clip_high, kl_coef, mean, grad_scale,
+    want_grad.  The gradient takes the place of the logits."""
+    logits, ids = _answers(pred, y)
+    if options.get("want_grad", True):
+        options.setdefault("dlogits", logits)
+    return sequence_loss.policy_loss(logits, ids, old_logp, advantage, **options)
 
 
 def activity_and_user_count(y):

@@ -317,7 +317,7 @@ class HierTCNModel:
     def train_step_device(self, xd, yd, md, st, lr, state_out=None, metrics8=None, y_score=None):
         """The step on device tensors, nothing read back: [global user count ->] forward + loss + scoring-layer backward ->
         [collective of the scoring layer's gradient, overlapped with] the rest of the backward -> [the other collectives] ->
-        TF-form Adam.  `metrics8` comes back summed over ranks (its loss is the global batch's, model.py:116-117)."""
+        TF-form Adam (or AdamW: args.optimizer).  `metrics8` comes back summed over ranks (its loss is the global batch's, model.py:116-117)."""
         from .distributed import GradientExchange, all_reduce_metrics
         eng = self.engine
         if getattr(self, "_exchange", None) is None:
@@ -333,7 +333,7 @@ class HierTCNModel:
         ex.after_scoring()
         eng.train_step_finish(xd, yd, md)
         ex.after_backward(xd, yd if self.hier else None)
-        eng.adam_step(float(lr), grad_scale=1.0)
+        eng.optimizer_step(float(lr), grad_scale=1.0)
         all_reduce_metrics(out["metrics8"])
         return out
 

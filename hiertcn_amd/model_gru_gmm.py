@@ -55,7 +55,7 @@ class GruGmmModel(TcnGmmModel):
 
     def __init__(self, args, params: Optional[dict] = None, name: str = "rnn_gmm", seed: int = 2):
         from .engine import check_supported
-        check_supported(args, loss_ok=("gmm_prob", "gmm_prob_max", "cross_entropy"))
+        check_supported(args, loss_ok=("gmm_prob", "gmm_prob_max", "cross_entropy"), optimizer_ok=("adam",))
         if not torch.cuda.is_available():
             raise HierTCNError("no GPU visible: the compute path is HIP-only (no CPU fallback)")
         self.args, self.name = args, name

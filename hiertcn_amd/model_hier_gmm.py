@@ -88,7 +88,7 @@ class HierGmmModel(TcnGmmModel):
     def __init__(self, args, params: Optional[dict] = None, name: str = "hier", seed: int = 2):
         from .engine import Engine, check_supported
         from .params import init_params as hier_init
-        check_supported(_scan_args(args))
+        check_supported(_scan_args(args), optimizer_ok=("adam",))
         if getattr(args, "loss", "gmm_prob") not in ("gmm_prob", "gmm_prob_max", "cross_entropy"):
             raise NotImplementedError(f"args.loss={args.loss!r}: the mixture low level evaluates 'gmm_prob' or 'gmm_prob_max' (loss.py:247-257)")
         if not torch.cuda.is_available():

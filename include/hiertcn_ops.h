@@ -9,7 +9,7 @@
  *     once as long as each has its own workspace and outputs.
  *   - returns 0 on success, otherwise a negative hiertcn_status (hiertcn.h); hiertcn_ops_last_error() holds this thread's message.
  *   - sizes are int64_t: tensors of more than 2^32 elements are fine.  Element strides are given where a tensor need not be contiguous.
- *   - results do not depend on timing: no atomics, every sum in a fixed order.
+ *   - results do not depend on timing: every sum has a fixed order.  (The one atomic, in long recurrences, numbers workgroups as they start.)
  */
 #ifndef HIERTCN_OPS_H_
 #define HIERTCN_OPS_H_
@@ -151,7 +151,8 @@ typedef struct {
 int hiertcn_adamw_step(const hiertcn_adamw_tensor_t* tensors, int64_t n, const hiertcn_adamw_t* a, void* stream);
 /* the values of 8-bit states: m_out[i], v_out[i] (HOST arrays of device float pointers, an entry may be NULL) */
 int hiertcn_adamw_moments(const hiertcn_adamw_tensor_t* tensors, int64_t n, float* const* m_out, float* const* v_out, void* stream);
-/* after another optimizer has changed a training handle's masters (hiertcn_train_arena 0): the 16-bit device copies, as hiertcn_adam_step refreshes them */
+/* after another optimizer has changed a training handle's masters (hiertcn_train_arena 0): the 16-bit device copies, as hiertcn_adam_step refreshes them.
+ * (A call on a handle: its message is in hiertcn_last_error().) */
 int hiertcn_train_masters_changed(hiertcn_handle_t h, void* stream);
 
 #ifdef __cplusplus

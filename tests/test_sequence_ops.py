@@ -315,3 +315,20 @@ def test_codes_keep_the_expectation_and_nearest_would_not():
         v = (SO.decode(q.astype(np.uint8), s, True) * b2 + (1 - b2)).astype(np.float32)
         q, s = SO.encode(np.sqrt(v), np.full(256, 1 << 15, np.uint32), True)
     assert (q == q0).all(), "rounding to nearest: two hundred steps do not move a code"
+
+
+def test_optimizer_arguments():
+    """--optimizer / --weight_decay: attributes only where given; refused where a model trains with Adam alone."""
+    from hiertcn_amd.args import make_args
+    from hiertcn_amd.engine import check_supported
+    assert not hasattr(make_args([]), "optimizer") and not hasattr(make_args([]), "weight_decay")
+    args = make_args(["--optimizer", "adamw", "--weight_decay", "0.1"])
+    assert args.optimizer == "adamw" and args.weight_decay == 0.1
+    check_supported(args)
+    with pytest.raises(NotImplementedError, match="optimizer"):
+        check_supported(args, optimizer_ok=("adam",))
+    del args.optimizer
+    with pytest.raises(NotImplementedError, match="weight_decay"):
+        check_supported(args)
+    with pytest.raises(SystemExit):
+        make_args(["--optimizer", "other"])
