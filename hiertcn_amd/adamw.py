@@ -14,6 +14,14 @@ from ._ops import need
 BLOCK = 256      # elements that share a scale of the 8-bit states
 
 
+def _apart(lists):
+    """Refuses two tensors of the lists that share memory: every one is written by waves of its own."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name, i) for name, ts in lists for i, t in enumerate(ts or ()) if t is not None and t.numel())
+    for (_, end, a, i), (start, _, b, j) in zip(spans, spans[1:]):
+        if start < end:
+            raise HierTCNError(f"{a}[{i}] and {b}[{j}] overlap")
+
+
 class AdamW:
     """params: fp32 masters (contiguous, on one GPU).  grads: where every step finds the gradients (fp32 / bf16 / fp16, None: no gradient) -- or give them to
     step().  copies: 16-bit tensors that receive the rounded parameters in the same pass (None entries: none).  weight_decay: one value, or one per
@@ -77,6 +85,7 @@ class AdamW:
             if self.state_bits == 8:
                 d.m_scale = need(m_scale[i], f"m_scale[{i}]", torch.float32, self.device, blocks).data_ptr()
                 d.v_scale = need(v_scale[i], f"v_scale[{i}]", torch.float32, self.device, blocks).data_ptr()
+        _apart((("params", self.params), ("copies", self.copies), ("m", m), ("v", v), ("m_scale", m_scale), ("v_scale", v_scale)))
         self.m, self.v, self.m_scale, self.v_scale = m, v, m_scale, v_scale
 
     def set_state(self, m, v, t: int, m_scale=None, v_scale=None):

@@ -147,7 +147,7 @@ typedef struct {
   int32_t state_bits;                  /* 32 or 8                                                                                     */
   int32_t reserved;
 } hiertcn_adamw_t;
-/* tensors: HOST array, read before the call returns */
+/* tensors: HOST array, read before the call returns.  The buffers of different tensors do not overlap (those of one are checked). */
 int hiertcn_adamw_step(const hiertcn_adamw_tensor_t* tensors, int64_t n, const hiertcn_adamw_t* a, void* stream);
 /* the values of 8-bit states: m_out[i], v_out[i] (HOST arrays of device float pointers, an entry may be NULL) */
 int hiertcn_adamw_moments(const hiertcn_adamw_tensor_t* tensors, int64_t n, float* const* m_out, float* const* v_out, void* stream);

@@ -158,3 +158,17 @@ def test_8_bit_states_follow_32_bit_ones():
     _, v = opt.moments()
     ratio = (v[0] / (g * g * (1 - B2 ** 3000))).double()
     assert abs(float(ratio.mean()) - 1) < 0.01 and float((ratio - 1).abs().max()) < 0.11, (float(ratio.mean()), float(ratio.min()), float(ratio.max()))
+
+
+def test_the_same_tensor_twice_is_refused():
+    from hiertcn_amd._lib import HierTCNError
+    from hiertcn_amd.adamw import AdamW
+    p = [torch.zeros(100, device="cuda"), torch.zeros(100, device="cuda")]
+    half = torch.zeros(100, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(HierTCNError, match="overlap"):
+        AdamW([p[0], p[0]])
+    with pytest.raises(HierTCNError, match="overlap"):
+        AdamW(p, copies=[half, half])
+    opt = AdamW(p)
+    with pytest.raises(HierTCNError, match="overlap"):
+        opt.set_state([opt.m[0], opt.m[0]], opt.v, 0)

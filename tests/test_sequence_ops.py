@@ -332,3 +332,13 @@ def test_optimizer_arguments():
         check_supported(args)
     with pytest.raises(SystemExit):
         make_args(["--optimizer", "other"])
+
+
+def test_optimizer_tensors_share_no_memory():
+    from hiertcn_amd.adamw import _apart
+    from hiertcn_amd._lib import HierTCNError
+    buf = torch.zeros(12)
+    _apart((("params", [buf[:4], buf[4:8]]), ("copies", [None, buf[8:]]), ("m", None), ("v", [buf[3:3]])))     # side by side, absent and empty ones
+    for lists in ([("params", [buf, buf])], [("params", [buf[:5]]), ("copies", [buf[4:]])], [("params", [buf[2:4], buf[9:], buf[:3]])]):
+        with pytest.raises(HierTCNError, match="overlap"):
+            _apart(lists)
