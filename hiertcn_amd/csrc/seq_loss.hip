@@ -7,6 +7,11 @@
 //   k_pairs / k_policy / k_logp   a few lanes a row: joins its parts, forms logp; the loss and c, in 64 bits (they are few)
 //   k_dlogits one pass over the logits: dz  (its first workgroup adds up the loss)
 // Masked rows are not read: their gradient rows are written as zeros.  All sums run in a fixed order.
+//
+// Bound by memory: the answered rows are read twice (c needs a whole row, a pair's needs two sequences), all gradient rows written once.  64 x 30 x 300000 bf16,
+// half of the rows answered: k_part 91 us for 0.58 GB (some of it in the last cache), k_policy 7, k_dlogits 279 for 1.73 GB (6.2 TB/s); 8 pairs x 30 x 300000
+// fp32: 33, 10, 113.  At 16 pairs x 20 x 20778 bf16 and below it is three launches of 4 to 8 us.  (A single pass that keeps the rows in registers while their
+// workgroups wait for one another is no faster: 461 us against 463 in two passes at the first of these, before the stores were taken past the caches.)
 #include <math.h>
 
 #include "ops.h"
@@ -445,22 +450,24 @@ __global__ __launch_bounds__(NT) void k_dlogits(RowsP p, Sums q) {
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------------------
 size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
-// parts of `elems` elements, or of as many more as MAX_PARTS asks for; a wave for a row that four rounds of a wave's loads cover
-Cut cut_of(int64_t V, int vec, int64_t elems) {
+// parts of `elems` elements, or of as many more as MAX_PARTS asks for.  A wave for a row that one round of its loads covers, or four rounds where there are rows
+// enough to fill the machine with waves; else a workgroup (12800 rows, both passes, us, wave / workgroup: 1000 bf16 25 / 42, 2000 32 / 51, 4000 49 / 65, 8000 84 / 88)
+Cut cut_of(int64_t R, int64_t V, int vec, int64_t elems) {
   if ((V + elems - 1) / elems > MAX_PARTS) elems = (V + MAX_PARTS - 1) / MAX_PARTS;
   Cut c;
   c.chunk = (elems + vec - 1) / vec;
   const int64_t nvec = V / vec;
   c.parts = (int)(nvec <= c.chunk ? 1 : (nvec + c.chunk - 1) / c.chunk);
-  c.tpr = nvec <= 256 ? 64 : NT;
+  c.tpr = c.parts == 1 && (nvec <= 256 || (nvec <= 1024 && R >= 4096)) ? 64 : NT;
   return c;
 }
+// (64 x 30 x 300000 bf16 and 16 x 30 x 300000 fp32: parts of 4096 to 16384 elements are within 2 % for the second pass, 32768 2 to 4 % slower)
 constexpr int64_t PART = 8192;
-// k_part's parts grow while 8192 of them are left
+// k_part's parts grow while 8192 of them are left (fewer prologues and joins: 148 us against 155 at 64 x 30 x 300000 bf16)
 Cut read_of(int64_t R, int64_t V, int vec) {
   int64_t elems = PART;
   while (elems < 4 * PART && R * ((V + 2 * elems - 1) / (2 * elems)) >= 8192) elems *= 2;
-  return cut_of(V, vec, elems);
+  return cut_of(R, V, vec, elems);
 }
 int64_t workgroups(const Cut& c, int64_t R) { return c.tpr == NT ? R * c.parts : (R + NT / 64 - 1) / (NT / 64); }
 int64_t counters_of(int64_t n, int64_t T) { return T <= COUNT_T ? (n + NT - 1) / NT : (n + NT / 64 - 1) / (NT / 64); }
@@ -516,7 +523,7 @@ int prepare(const hiertcn_rows_t* in, bool grad, RowsP& p, int& vec) {
   vec = 16 / es;
   if (a.dlogits && (((uintptr_t)a.logits - (uintptr_t)a.dlogits) % 16 || (a.ld - a.dld) % vec)) vec = 1;
   p.read = read_of(p.R, a.V, vec);
-  p.write = cut_of(a.V, vec, PART);
+  p.write = cut_of(p.R, a.V, vec, PART);
   p.counters = 0;
   workspace_of(a.n, a.T, a.V, &p);
   if (workgroups(p.read, p.R) + a.n > 0x7fffffffll || workgroups(p.write, p.R) + a.n > 0x7fffffffll) return ops_fail(HIERTCN_ERR_INVALID, "n * T * V is too large for one launch");

@@ -238,3 +238,34 @@ def test_offsets_behind_2_to_the_32():
     p = np.exp(3.0) / (V - 1 + np.exp(3.0))
     assert abs(float(z[1, T - 1, 199999]) + (1 - p)) < 2 ** -8 and abs(float(z[1, T - 1, 5]) - p / np.exp(3.0)) < 2 ** -8 * p
     assert (z[0, 0] == 0).all() and (z[1, T - 2] == 0).all()
+
+
+@pytest.mark.parametrize("V", [2045, 4001, 8190])
+def test_many_rows_of_some_thousand_items(V):
+    """4160 rows (a wave takes a row; four rounds of its loads at the longest), against the same rows in two batches of fewer (a workgroup takes a row from 2049
+    items on): both within the bounds of the formula; every 97th row is compared with 64 bits."""
+    from hiertcn_amd.sequence_loss import policy_loss, sequence_logp
+    n, T = 1040, 4
+    g = torch.Generator(device="cuda").manual_seed(V)
+    z = (2 * torch.randn(n, T, V, generator=g, device="cuda")).clamp(-10, 10).to(torch.bfloat16)
+    ids = torch.randint(1, V, (n, T), generator=g, device="cuda", dtype=torch.int32)
+    ids[::3, 2:] = 0
+    lp = sequence_logp(z, ids)
+    parts = torch.cat([sequence_logp(z[:520], ids[:520]), sequence_logp(z[520:], ids[520:])])
+    rows = torch.arange(0, n, 97)
+    want = SO.rows(n64(z[rows]), ids[rows].cpu().numpy())
+    # (a lane of 64 sums up to 128 elements: 96 half steps more than the 32 that the bound counts)
+    allowed = 1.01 * (want["logp_err"] + 96 * HALF[torch.float32]) + HALF[torch.float32] * np.abs(want["logp"])
+    for got in (lp, parts):
+        assert (np.abs(n64(got[rows]) - want["logp"]) <= allowed).all()
+    adv = torch.randn(n, generator=g, device="cuda")
+    out = policy_loss(z, ids, lp, adv, grad_scale=float(n))                  # ratios of one: c = -A / answers
+    p = torch.softmax(z[rows].double(), -1)
+    hot = torch.zeros_like(p).scatter_(-1, ids[rows].long()[..., None], 1.0)
+    live = (ids[rows] > 0).double()
+    c = (-adv[rows].double()[:, None] / (ids[rows] > 0).sum(1, keepdim=True)) * live
+    ref = c[..., None] * (hot - p)
+    err = (out["dlogits"][rows].double() - ref).abs()
+    # relative: (120 + 96) half steps of the sum and 2 (20 + 8) of the exponential, a ratio off by lp's rounding (16 half steps), bf16's half step
+    assert (err <= ref.abs() * (HALF[torch.bfloat16] + 400 * HALF[torch.float32]) + 400 * HALF[torch.float32] * c.abs()[..., None]).all(), float(err.max())
+    assert (out["dlogits"][::3, 2:] == 0).all()
