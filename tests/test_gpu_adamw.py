@@ -172,3 +172,47 @@ def test_the_same_tensor_twice_is_refused():
     opt = AdamW(p)
     with pytest.raises(HierTCNError, match="overlap"):
         opt.set_state([opt.m[0], opt.m[0]], opt.v, 0)
+
+
+def test_elements_behind_2_to_the_32():
+    """A tensor of 2^32 + 700 elements: its last blocks and its first ones step as the formula says, and their random bits take the high word of the index."""
+    from hiertcn_amd.adamw import AdamW
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("60 GiB of device memory")
+    n, tail, lr = 2 ** 32 + 700, 956, 1e-2
+    p = torch.full((n,), 0.5, device="cuda")
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    rng = np.random.default_rng(4)
+    ends = torch.tensor(rng.standard_normal((2, tail)), dtype=torch.float32).to(torch.bfloat16)
+    g[:tail], g[n - tail:] = ends[0].cuda(), ends[1].cuda()
+    opt = AdamW([p], [g], lr=lr, betas=(B1, B2), eps=E, state_bits=8, seed=9)
+    opt.step()
+    opt.step()
+    start = n - tail                                       # a multiple of 256: whole blocks, on both sides of 2^32
+    assert start % 256 == 0 and start < 2 ** 32 < n
+    for at, grad in ((0, ends[0]), (start, ends[1])):
+        q = np.full(tail, 0.5, np.float32)
+        qm, qv, blocks = np.zeros(tail, np.int8), np.zeros(tail, np.uint8), -(-tail // 256)
+        sm, sv = np.zeros(blocks, np.float32), np.zeros(blocks, np.float32)
+        for t in (1, 2):
+            whole = SO.mix
+            try:                                           # the oracle's bits of elements at .. at + tail - 1
+                SO.mix = lambda numel, tensor, t, seed, at=at: _bits(at + np.arange(numel, dtype=np.uint64), t, seed)
+                q, qm, qv, sm, sv = SO.adamw8(q, grad.float().numpy(), qm, qv, sm, sv, t, lr, B1, B2, E, 0.0, 9, 0)
+            finally:
+                SO.mix = whole
+        b0 = at // 256
+        for got, want in ((opt.m[0][at:at + tail], qm), (opt.v[0][at:at + tail], qv), (opt.m_scale[0][b0:b0 + blocks], sm), (opt.v_scale[0][b0:b0 + blocks], sv)):
+            assert np.array_equal(got.cpu().numpy(), want), at
+        assert (np.abs(p[at:at + tail].cpu().numpy() - q) <= 4 * EPS * (np.abs(q) + 1e-2)).all()
+    assert (p[tail:start] == 0.5).all()
+
+
+def _bits(e, t, seed):
+    u = np.uint32
+    with np.errstate(over="ignore"):
+        key = u((seed * 0x9E3779B1 + t * 0x6A09E667) & 0xFFFFFFFF) + (e >> np.uint64(32)).astype(u) * u(0x1F83D9AB)
+        x = e.astype(u) * u(0x9E3779B1) + key
+        x = (x ^ (x >> u(16))) * u(0x3C6EF373)
+        x = (x ^ (x >> u(15))) * u(0x510E527F)
+        return x ^ (x >> u(16))

@@ -225,3 +225,40 @@ def test_training_with_adamw_from_the_command_line():
         quiet = g[k] == 0
         assert np.abs(after[k] - before[k] * (1 - 1e-5))[quiet].max(initial=0.0) <= 8 * U * np.abs(before[k]).max(), k
     model.engine.close()
+
+
+def test_calls_on_two_streams_at_once():
+    """Long recurrences (whose workgroups hand states to one another), losses and steps on two streams, queued without a wait between them: what each gives alone."""
+    from hiertcn_amd.glr import glr_scan, glr_scan_backward
+    from hiertcn_amd.sequence_loss import policy_loss
+    g = torch.Generator(device="cuda").manual_seed(11)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    B, T, D, n, V = 3, 9001, 130, 12, 30011
+
+    def inputs():
+        return dict(p=rn(B, T, 2 * D).to(torch.bfloat16), dh=rn(B, T, D).to(torch.bfloat16), s=rn(B, D), z=rn(n, 5, V), ids=torch.randint(0, V, (n, 5), generator=g, device="cuda", dtype=torch.int32),
+                    old=rn(n, 5) - 10, adv=rn(n))
+
+    def work(q):
+        gate, cand = q["p"][..., :D], q["p"][..., D:]
+        h, last, record = glr_scan(gate, cand, q["s"], want_record=True)
+        dg, dc, ds = glr_scan_backward(gate, cand, q["dh"], record)
+        out = policy_loss(q["z"], q["ids"], q["old"], q["adv"], ref_logp=q["old"], kl_coef=0.1)
+        return h, last, dg, dc, ds, out["loss"], out["dlogits"]
+    sets = [inputs(), inputs()]
+    alone = []
+    for q in sets:
+        alone.append(work(q))
+        torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(6):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(work(sets[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for res in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(res, alone[k])), k
