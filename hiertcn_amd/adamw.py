@@ -26,14 +26,15 @@ class AdamW:
     """params: fp32 masters (contiguous, on one GPU).  grads: where every step finds the gradients (fp32 / bf16 / fp16, None: no gradient) -- or give them to
     step().  copies: 16-bit tensors that receive the rounded parameters in the same pass (None entries: none).  weight_decay: one value, or one per
     tensor.  state_bits 32: m, v fp32 (8 bytes a parameter); 8: codes with a scale per 256 elements (2 bytes a parameter), rounded at random such that
-    the expected state is exact -- `seed` and the step number determine the random bits, so runs repeat.
+    the expected state is exact -- `seed` and the step number determine the random bits, so runs repeat.  state: (m, v) or (m, v, m_scale, v_scale), taken as
+    set_state takes them, in place of zeros of the optimizer's own.
 
     The step number is the object's (`t`), so a step cannot be captured into a graph (it would replay with the same bias corrections): it is refused
     there, as the framework's graphs leave Adam outside."""
 
     def __init__(self, params: Sequence[torch.Tensor], grads: Optional[Sequence[Optional[torch.Tensor]]] = None, lr: float = 1e-3, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: Union[float, Sequence[float]] = 0.0, state_bits: int = 32,
-                 copies: Optional[Sequence[Optional[torch.Tensor]]] = None, seed: int = 0):
+                 copies: Optional[Sequence[Optional[torch.Tensor]]] = None, seed: int = 0, state: Optional[Sequence] = None):
         if state_bits not in (8, 32):
             raise HierTCNError(f"state_bits {state_bits}: 8 or 32")
         self.params: List[torch.Tensor] = list(params)
@@ -57,11 +58,12 @@ class AdamW:
                     raise HierTCNError(f"copies[{i}]: a bfloat16 or float16 tensor")
                 d.copy, d.copy_dtype = need(c, f"copies[{i}]", c.dtype, self.device, p.shape).data_ptr(), _ops.DTYPE[c.dtype]
         self.set_weight_decay(weight_decay)
-        zeros = lambda dt, block=1: [torch.zeros(-(-p.numel() // block), dtype=dt, device=self.device) for p in self.params]  # noqa: E731
-        if state_bits == 32:
-            self._attach(zeros(torch.float32), zeros(torch.float32), None, None)
+        if state is not None:
+            self._take(state)
         else:
-            self._attach(zeros(torch.int8), zeros(torch.uint8), zeros(torch.float32, BLOCK), zeros(torch.float32, BLOCK))
+            zeros = lambda dt, block=1: [torch.zeros(-(-p.numel() // block), dtype=dt, device=self.device) for p in self.params]  # noqa: E731
+            self._attach(*((zeros(torch.float32), zeros(torch.float32), None, None) if state_bits == 32 else
+                           (zeros(torch.int8), zeros(torch.uint8), zeros(torch.float32, BLOCK), zeros(torch.float32, BLOCK))))
         self.grads = None
         if grads is not None:
             self._bind(grads)
@@ -90,13 +92,16 @@ class AdamW:
 
     def set_state(self, m, v, t: int, m_scale=None, v_scale=None):
         """Takes flat tensors as the states THEMSELVES (no copy): fp32 moments, or int8 / uint8 codes with their scales [ceil(numel / 256)]; t: steps taken."""
-        lists = [list(x) if x is not None else None for x in (m, v, m_scale, v_scale)]
-        if any(x is not None and len(x) != len(self.params) for x in lists) or None in lists[:2] or (self.state_bits == 8) != (None not in lists[2:]):
-            raise HierTCNError("one m and one v per parameter, and a scale of each with 8-bit states only")
         if int(t) < 0:
             raise HierTCNError(f"t = {t}")
-        self._attach(*lists)
+        self._take((m, v, m_scale, v_scale))
         self.t = int(t)
+
+    def _take(self, state):
+        lists = [list(x) if x is not None else None for x in (*state, None, None)[:4]]
+        if any(x is not None and len(x) != len(self.params) for x in lists) or None in lists[:2] or (self.state_bits == 8) != (None not in lists[2:]):
+            raise HierTCNError("one m and one v per parameter, and a scale of each with 8-bit states only")
+        self._attach(*lists)
 
     def state_dict(self) -> dict:
         """t, seed and the states on the host (checkpoints)."""

@@ -591,12 +591,12 @@ class Engine:
             from . import _ops
             from .adamw import AdamW
             _ops.bind(self.lib)
-            self._adamw = AdamW([self._arena(0)], [self._arena(1)])
+            self._adamw = AdamW([self._arena(0)], [self._arena(1)], state=([self._arena(2)], [self._arena(3)]))
         opt, t = self._adamw, C.c_int64(0)
         self._ck(self.lib.hiertcn_adam_time(self._h, C.byref(t), None))
         opt.betas, opt.eps = (float(beta1), float(beta2)), float(eps)
         opt.set_weight_decay(weight_decay)
-        opt.set_state([self._arena(2)], [self._arena(3)], t.value)
+        opt.t = t.value
         opt.step(lr=lr, grad_scale=grad_scale)
         t.value += 1
         self._ck(self.lib.hiertcn_adam_time(self._h, None, C.byref(t)))

@@ -216,3 +216,20 @@ def _bits(e, t, seed):
         x = (x ^ (x >> u(16))) * u(0x3C6EF373)
         x = (x ^ (x >> u(15))) * u(0x510E527F)
         return x ^ (x >> u(16))
+
+
+def test_states_of_the_callers_own():
+    from hiertcn_amd._lib import HierTCNError
+    from hiertcn_amd.adamw import AdamW
+    params, grads, _ = tensors([300, 7], 12)
+    twin = [p.clone() for p in params]
+    m, v = ([torch.zeros_like(p) for p in params] for _ in range(2))
+    a, b = AdamW(params, grads, state=(m, v)), AdamW(twin, grads)
+    for _ in range(2):
+        a.step()
+        b.step()
+    assert all(torch.equal(x, y) for x, y in zip(params + m + v, twin + b.m + b.v)) and a.m[0] is m[0]
+    with pytest.raises(HierTCNError):
+        AdamW(params, grads, state=(m, v), state_bits=8)
+    with pytest.raises(HierTCNError):
+        AdamW(params, grads, state=(m[:1], v))
