@@ -50,7 +50,8 @@ class AdamW:
         self.lr, self.betas, self.eps, self.state_bits, self.seed, self.t = float(lr), (float(betas[0]), float(betas[1])), float(eps), state_bits, int(seed), 0
         self.copies = copies
         self._desc = (_ops.AdamwTensor * n)()
-        self._flat = [torch.Size([p.numel()]) for p in self.params]
+        self._flat_numel = [p.numel() for p in self.params]
+        self._flat = [torch.Size([k]) for k in self._flat_numel]
         for i, (p, c, d) in enumerate(zip(self.params, copies, self._desc)):
             d.numel, d.param, d.index = p.numel(), p.data_ptr(), i
             if c is not None:
@@ -80,14 +81,15 @@ class AdamW:
         self.weight_decay = decay
 
     def _attach(self, m, v, m_scale, v_scale):
+        """All of it, or (an exception) none."""
         dm, dv = (torch.float32, torch.float32) if self.state_bits == 32 else (torch.int8, torch.uint8)
-        for i, (p, d) in enumerate(zip(self.params, self._desc)):
-            k, blocks = torch.Size([p.numel()]), torch.Size([-(-p.numel() // BLOCK)])
-            d.m, d.v = need(m[i], f"m[{i}]", dm, self.device, k).data_ptr(), need(v[i], f"v[{i}]", dv, self.device, k).data_ptr()
-            if self.state_bits == 8:
-                d.m_scale = need(m_scale[i], f"m_scale[{i}]", torch.float32, self.device, blocks).data_ptr()
-                d.v_scale = need(v_scale[i], f"v_scale[{i}]", torch.float32, self.device, blocks).data_ptr()
+        names = (("m", m, dm, 1), ("v", v, dv, 1)) + ((("m_scale", m_scale, torch.float32, BLOCK), ("v_scale", v_scale, torch.float32, BLOCK)) if self.state_bits == 8 else ())
+        found = [[need(t, f"{name}[{i}]", dt, self.device, torch.Size([-(-k // block)])).data_ptr() for i, (t, k) in enumerate(zip(ts, self._flat_numel))]
+                 for name, ts, dt, block in names]
         _apart((("params", self.params), ("copies", self.copies), ("m", m), ("v", v), ("m_scale", m_scale), ("v_scale", v_scale)))
+        for (name, _, _, _), ptrs in zip(names, found):
+            for d, ptr in zip(self._desc, ptrs):
+                setattr(d, name, ptr)
         self.m, self.v, self.m_scale, self.v_scale = m, v, m_scale, v_scale
 
     def set_state(self, m, v, t: int, m_scale=None, v_scale=None):
@@ -123,15 +125,16 @@ class AdamW:
         self.t, self.seed = int(state["t"]), int(state["seed"])
 
     def _bind(self, grads):
+        """All of them, or (an exception) none."""
         if len(grads) != len(self.params):
             raise HierTCNError(f"{len(self.params)} parameters, {len(grads)} gradients")
-        for i, (p, g, d) in enumerate(zip(self.params, grads, self._desc)):
-            if g is None:
-                d.grad = None
-                continue
-            if not isinstance(g, torch.Tensor) or g.dtype not in _ops.DTYPE:
+        found = []
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            if g is not None and (not isinstance(g, torch.Tensor) or g.dtype not in _ops.DTYPE):
                 raise HierTCNError(f"grads[{i}]: a float32, bfloat16 or float16 tensor")
-            d.grad, d.grad_dtype = need(g, f"grads[{i}]", g.dtype, self.device, p.shape).data_ptr(), _ops.DTYPE[g.dtype]
+            found.append((None, 0) if g is None else (need(g, f"grads[{i}]", g.dtype, self.device, p.shape).data_ptr(), _ops.DTYPE[g.dtype]))
+        for d, (ptr, dtype) in zip(self._desc, found):
+            d.grad, d.grad_dtype = ptr, dtype
 
     def step(self, grads: Optional[Sequence[Optional[torch.Tensor]]] = None, lr: Optional[float] = None, grad_scale: Union[float, torch.Tensor] = 1.0):
         """One step.  grads: this step's (default: the buffers given to the constructor); a parameter without one is left as it is.  grad_scale multiplies

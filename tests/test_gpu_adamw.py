@@ -233,3 +233,24 @@ def test_states_of_the_callers_own():
         AdamW(params, grads, state=(m, v), state_bits=8)
     with pytest.raises(HierTCNError):
         AdamW(params, grads, state=(m[:1], v))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_binding_leaves_the_optimizer_as_it_was(bits):
+    """Gradients or states that are refused half-way: the next step works on the ones from before, not on a part of the refused ones."""
+    from hiertcn_amd._lib import HierTCNError
+    from hiertcn_amd.adamw import AdamW
+    params, grads, _ = tensors([500, 60], 13)
+    twin = [p.clone() for p in params]
+    a, b = AdamW(params, grads, state_bits=bits, seed=3), AdamW(twin, grads, state_bits=bits, seed=3)
+    bad = [torch.full((500,), float("nan"), device="cuda"), torch.zeros(61, device="cuda")]
+    with pytest.raises(HierTCNError, match=r"grads\[1\]"):
+        a.step(bad)
+    z = [torch.zeros_like(x) for x in a.m]
+    kw = {} if bits == 32 else dict(m_scale=[torch.zeros_like(x) for x in a.m_scale], v_scale=[torch.zeros_like(x) for x in a.v_scale])
+    with pytest.raises(HierTCNError, match=r"v\[1\]"):
+        a.set_state(z, [torch.zeros_like(a.v[0]), torch.zeros_like(a.v[1])[:-1]], 0, **kw)
+    assert a.t == 0
+    a.step()
+    b.step()
+    assert all(torch.equal(x, y) for x, y in zip(params + a.m + a.v, twin + b.m + b.v)) and not any(x.any() for x in z)
