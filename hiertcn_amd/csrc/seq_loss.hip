@@ -200,20 +200,21 @@ __device__ __forceinline__ float logit(const hiertcn_rows_t& a, int64_t off) {
   return a.dtype == HIERTCN_FP32 ? static_cast<const float*>(a.logits)[off] : ops_h2f(static_cast<const uint16_t*>(a.logits)[off], a.dtype);
 }
 
-// p.lanes neighbours a row: logp from its parts, (m, 1 / s) kept for the gradient.  false: masked, or nothing but -inf
-__device__ bool finish_row(const RowsP& p, int64_t r, double& logp) {
+// p.lanes neighbours a row: logp from its parts, (m, 1 / s) kept for the gradient.  ROW_EMPTY: answered, but nothing but -inf
+enum Row { ROW_MASKED, ROW_EMPTY, ROW_LIVE };
+__device__ Row finish_row(const RowsP& p, int64_t r, double& logp) {
   int32_t y;
   logp = 0.0;
-  if (!answered(p.a, r, y)) return false;
+  if (!answered(p.a, r, y)) return ROW_MASKED;
   const int i = threadIdx.x & (p.lanes - 1);
   const float2 x = i < p.read.parts ? p.part[r * p.read.parts + i] : make_float2(-INFINITY, 0.f);
   const float z = logit(p.a, r * p.a.ld + y);
   float m = x.x, s = x.y;
   for (int d = p.lanes >> 1; d; d >>= 1) join(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
   if (i == 0) p.stat[r] = make_float2(m, 1.f / s);
-  if (m == -INFINITY && s == 0.f) return false;
+  if (m == -INFINITY && s == 0.f) return ROW_EMPTY;
   logp = ((double)z - ref_of(m)) - log((double)s);
-  return true;
+  return ROW_LIVE;
 }
 // the row of this thread's lanes, of n rows beginning at the workgroup's first
 __device__ __forceinline__ int64_t row_here(const RowsP& p) { return (int64_t)blockIdx.x * (NT / p.lanes) + threadIdx.x / p.lanes; }
@@ -275,17 +276,20 @@ __global__ __launch_bounds__(PAIR_NT) void k_pairs(RowsP p, hiertcn_preference_t
   const hiertcn_rows_t& a = p.a;
   const int64_t P = a.n / 2;
   const int64_t first = threadIdx.x / p.lanes, step = PAIR_NT / p.lanes;
+  const float ref[2] = {q.ref[blockIdx.x], q.ref[blockIdx.x + P]};
   double x[4] = {};                                            // sums of logp, numbers of answers
-  for (int64_t i = first; i < 2 * a.T; i += step) {
+  uint64_t kept = 0;                                           // bit k: the k-th of this thread's rows has a distribution
+  int k = 0;
+  for (int64_t i = first; i < 2 * a.T; i += step, k++) {
     const int side = i >= a.T;
     const int64_t r = side ? (blockIdx.x + P) * a.T + (i - a.T) : blockIdx.x * a.T + i;
     double lp;
-    const bool live = finish_row(p, r, lp);
+    const Row row = finish_row(p, r, lp);
     if (first_lane(p)) {
-      int32_t y;
       a.logp[r] = (float)lp;
-      p.coef[r] = live ? 1.f : 0.f;
-      const double one = answered(a, r, y) ? 1.0 : 0.0;
+      if (k < 64) kept |= (uint64_t)(row == ROW_LIVE) << k;
+      else p.coef[r] = row == ROW_LIVE ? 1.f : 0.f;
+      const double one = row != ROW_MASKED ? 1.0 : 0.0;
       x[0] += side ? 0.0 : lp;
       x[1] += side ? lp : 0.0;
       x[2] += side ? 0.0 : one;
@@ -293,11 +297,11 @@ __global__ __launch_bounds__(PAIR_NT) void k_pairs(RowsP p, hiertcn_preference_t
     }
   }
   block_sum<PAIR_NT / 64>(x);
-  double s[2];
-  for (int side = 0; side < 2; side++) s[side] = q.average ? (x[2 + side] > 0 ? x[side] / x[2 + side] : 0.0) : x[side];
   __shared__ float c[2];
   if (threadIdx.x == 0) {                                      // one wave: 64-bit exponentials in all 16 cost 5 us
-    const double D = (s[0] - q.ref[blockIdx.x]) - (s[1] - q.ref[blockIdx.x + P]);
+    double s[2];
+    for (int side = 0; side < 2; side++) s[side] = q.average ? (x[2 + side] > 0 ? x[side] / x[2 + side] : 0.0) : x[side];
+    const double D = (s[0] - ref[0]) - (s[1] - ref[1]);
     double loss, slope;
     pair_of(q, D, loss, slope);
     c[0] = coef_of(p, q, slope, 0, x[2]);
@@ -309,10 +313,12 @@ __global__ __launch_bounds__(PAIR_NT) void k_pairs(RowsP p, hiertcn_preference_t
   }
   __syncthreads();
   if (!first_lane(p)) return;
-  for (int64_t i = first; i < 2 * a.T; i += step) {            // (this thread's own rows of the loop above)
+  k = 0;
+  for (int64_t i = first; i < 2 * a.T; i += step, k++) {       // (this thread's own rows of the loop above)
     const int side = i >= a.T;
     const int64_t r = side ? (blockIdx.x + P) * a.T + (i - a.T) : blockIdx.x * a.T + i;
-    p.coef[r] = p.coef[r] != 0.f ? c[side] : 0.f;
+    const bool live = k < 64 ? kept >> k & 1 : p.coef[r] != 0.f;
+    p.coef[r] = live ? c[side] : 0.f;
   }
 }
 
@@ -352,7 +358,7 @@ __global__ __launch_bounds__(NT) void k_policy(RowsP p, hiertcn_policy_t q) {
   double x[3] = {};
   if (r < p.R) {
     double lp;
-    const bool live = finish_row(p, r, lp);
+    const bool live = finish_row(p, r, lp) == ROW_LIVE;
     if (first_lane(p)) {
       Answer o{0.0, 0.0, 0.0, 0.0};
       if (live) o = answer_of(q, a.T, r, lp, 1.0 / (q.mean == 0 ? total[0] * p.count[r / a.T] : total[0]));

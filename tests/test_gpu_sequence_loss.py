@@ -269,3 +269,29 @@ def test_many_rows_of_some_thousand_items(V):
     # relative: (120 + 96) half steps of the sum and 2 (20 + 8) of the exponential, a ratio off by lp's rounding (16 half steps), bf16's half step
     assert (err <= ref.abs() * (HALF[torch.bfloat16] + 400 * HALF[torch.float32]) + 400 * HALF[torch.float32] * c.abs()[..., None]).all(), float(err.max())
     assert (out["dlogits"][::3, 2:] == 0).all()
+
+
+def test_a_pair_of_very_long_sequences():
+    """40000 answers a sequence of 9 items: more rows than a thread of the pair's workgroup keeps bits for.  A row's logp is within 2^-24 (120 + 2 (4 + 20) + 60) of
+    itself, D within 2 T of that (1.1 at the worst), its slope within beta^2 / 4 of D's: 1e-3 of beta at beta = 1e-3 (with the rounding of c and p)."""
+    from hiertcn_amd.sequence_loss import preference_loss
+    T, V, beta = 40000, 9, 1e-3
+    g = torch.Generator(device="cuda").manual_seed(2)
+    z = (2 * torch.randn(2, T, V, generator=g, device="cuda")).clamp(-10, 10)
+    ids = torch.randint(0, V, (2, T), generator=g, device="cuda", dtype=torch.int32)
+    z[1, 5], z[0, 39999] = -float("inf"), -float("inf")                      # rows of no distribution, near both ends
+    ids[1, 5], ids[0, 39999] = 2, 3
+    ref = torch.tensor([-80000.0, -79900.0], device="cuda")
+    out = preference_loss(z, ids, ref, beta=beta, grad_scale=1000.0)
+    z64, hot = z.double().cpu(), torch.nn.functional.one_hot(ids.long().cpu(), V).double()
+    ok = (ids.cpu() > 0) & torch.isfinite(z64[..., 0])
+    lp = torch.where(ok, (torch.log_softmax(torch.nan_to_num(z64, neginf=0.0), -1) * hot).sum(-1), torch.zeros(()).double())
+    s = lp.sum(1)
+    bound = 228 * 2.0 ** -24 * T
+    assert ((out["seq_logp"].double().cpu() - s).abs() <= bound + 2.0 ** -24 * s.abs()).all()
+    D = float((s[0] - ref[0].double().cpu()) - (s[1] - ref[1].double().cpu()))
+    c = 1000.0 * beta * (1 / (1 + np.exp(-beta * D)) - 1.0)
+    want = torch.stack([c * (hot[0] - torch.softmax(z64[0], -1)), -c * (hot[1] - torch.softmax(z64[1], -1))])
+    want = torch.where(ok[..., None], want, torch.zeros(()).double())
+    got = out["dlogits"].double().cpu()
+    assert (got[~ok] == 0).all() and ((got - want)[ok].abs() <= 1e-3 * abs(c) + 1000.0 * beta ** 2 / 4 * 2 * bound).all()
