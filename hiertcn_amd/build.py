@@ -33,6 +33,60 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+NO_NAN_SOURCES = ("score.hip", "score_x3.hip", "score_x3w.hip")
+
+
+def _flags_of(src: str, extra=()):
+    # score.hip: logits are finite or -inf by construction; without NaN-honouring fmaxf needs no
+    # canonicalising v_max on MFMA results (cdna_hip_programming.md, attention 'Pitfalls')
+    return [*FLAGS, *(["-fno-honor-nans"] if src in NO_NAN_SOURCES else []), *extra]
+
+
+def _compile(sources, obj_dir: str, extra=(), force: bool = False, verbose: bool = False):
+    """Objects of `sources` in obj_dir -> (their paths, whether any was compiled).  An object is stale when its source or a header is newer, and ALL of a
+    directory are when the flags they were compiled with (its objects.flags) are not today's: a changed flag leaves no old object behind."""
+    os.makedirs(obj_dir, exist_ok=True)
+    hipcc, headers = _hipcc(), _headers()
+    stamp, flagset = os.path.join(obj_dir, "objects.flags"), "\n".join(" ".join([src, *_flags_of(src, extra)]) for src in sources)
+    try:
+        with open(stamp) as f:
+            same = f.read() == flagset
+    except OSError:
+        same = False
+    jobs, objs = [], []
+    for src in sources:
+        s, o = os.path.join(CSRC, src), os.path.join(obj_dir, src.replace(".hip", ".o"))
+        objs.append(o)
+        if force or not same or _stale(o, [s] + headers + _ops_headers(src)):
+            jobs.append((src, s, o))
+    if not same and os.path.exists(stamp):
+        os.remove(stamp)                      # (until all of them are: a run that fails or is stopped half-way starts over)
+
+    def cc(job):
+        src, s, o = job
+        cmd = [hipcc, *_flags_of(src, extra), "-c", s, "-o", o]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("hipcc failed: %s\n%s\n%s" % (" ".join(cmd), r.stdout, r.stderr))
+        if verbose and r.stderr.strip():
+            print(r.stderr, file=sys.stderr)
+
+    if jobs:
+        with ThreadPoolExecutor(max_workers=min(6, len(jobs))) as ex:
+            list(ex.map(cc, jobs))
+    if not same:
+        with open(stamp, "w") as f:
+            f.write(flagset)
+    return objs, bool(jobs)
+
+
+def _link(lib: str, objs):
+    # nothing but the HIP runtime: every kernel of the library, the plain GEMMs of the backward pass included (csrc/gemm.hip), is its own
+    r = subprocess.run([_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib, *objs], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("link failed: %s\n%s" % (r.stdout, r.stderr))
+
+
 LIB_F16 = os.path.join(HERE, "libhiertcn_gfx950_f16.so")
 
 
@@ -56,37 +110,13 @@ def _mentions_ablation(src: str) -> bool:
 
 def build_ablation(force: bool = False) -> str:
     build_lib(False)
-    hipcc = _hipcc()
-    obj_dir = os.path.join(HERE, "build", "ablation")
-    os.makedirs(obj_dir, exist_ok=True)
-    headers = _headers()
-    jobs, objs = [], []
-    for src in SOURCES + ABLATION_EXTRA_SOURCES:
-        if src in ABLATION_EXTRA_SOURCES or _mentions_ablation(src):
-            s, o = os.path.join(CSRC, src), os.path.join(obj_dir, src.replace(".hip", ".o"))
-            if force or _stale(o, [s] + headers):
-                jobs.append((s, o))
-            objs.append(o)
-        else:   # no ablation content: the shipped library's object
-            objs.append(os.path.join(HERE, "build", src.replace(".hip", ".o")))
-
-    def cc(job):
-        s, o = job
-        per_file = ["-fno-honor-nans"] if s.endswith(NO_NAN_SOURCES) else []
-        r = subprocess.run([hipcc, *FLAGS, *per_file, "-DHIERTCN_ABLATION=1", "-c", s, "-o", o], capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("hipcc failed: %s\n%s" % (s, r.stderr))
-    if jobs:
-        with ThreadPoolExecutor(max_workers=min(6, len(jobs))) as ex:
-            list(ex.map(cc, jobs))
-    if force or jobs or _stale(LIB_ABLATION, objs):
-        r = subprocess.run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_ABLATION, *objs], capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("link failed: %s\n%s" % (r.stdout, r.stderr))
+    # a source without ablation content: the shipped library's object
+    own = [src for src in SOURCES + ABLATION_EXTRA_SOURCES if src in ABLATION_EXTRA_SOURCES or _mentions_ablation(src)]
+    objs, built = _compile(own, os.path.join(OBJ, "ablation"), ["-DHIERTCN_ABLATION=1"], force)
+    objs += [os.path.join(OBJ, src.replace(".hip", ".o")) for src in SOURCES if src not in own]
+    if force or built or _stale(LIB_ABLATION, objs):
+        _link(LIB_ABLATION, objs)
     return LIB_ABLATION
-
-
-NO_NAN_SOURCES = ("score.hip", "score_x3.hip", "score_x3w.hip")
 
 
 def _headers():
@@ -124,84 +154,35 @@ def build_testhooks(force: bool = False) -> str:
     shipped libraries have none).  Same objects as the shipped library except the few sources that hold a switch.  Loaded only by
     tests/tools/persist_timeout_probe.py through HIERTCN_LIB."""
     build_lib(False)
-    hipcc = _hipcc()
-    obj_dir = os.path.join(HERE, "build", "testhooks")
-    os.makedirs(obj_dir, exist_ok=True)
-    headers = _headers()
-    objs = []
-    rebuilt = False
-    for src in SOURCES:
-        if src in TESTHOOK_SOURCES:
-            s, o = os.path.join(CSRC, src), os.path.join(obj_dir, src.replace(".hip", ".o"))
-            if force or _stale(o, [s] + headers):
-                r = subprocess.run([hipcc, *FLAGS, "-DHIERTCN_TEST_HOOKS=1", "-c", s, "-o", o], capture_output=True, text=True)
-                if r.returncode != 0:
-                    raise RuntimeError("hipcc failed: %s\n%s" % (s, r.stderr))
-                rebuilt = True
-            objs.append(o)
-        else:
-            objs.append(os.path.join(HERE, "build", src.replace(".hip", ".o")))
-    if force or rebuilt or _stale(LIB_TESTHOOKS, objs):
-        r = subprocess.run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_TESTHOOKS, *objs], capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("link failed: %s\n%s" % (r.stdout, r.stderr))
+    objs, built = _compile(TESTHOOK_SOURCES, os.path.join(OBJ, "testhooks"), ["-DHIERTCN_TEST_HOOKS=1"], force)
+    objs += [os.path.join(OBJ, src.replace(".hip", ".o")) for src in SOURCES if src not in TESTHOOK_SOURCES]
+    if force or built or _stale(LIB_TESTHOOKS, objs):
+        _link(LIB_TESTHOOKS, objs)
     return LIB_TESTHOOKS
 
 
 def build_lib(force: bool = False, verbose: bool = False, extra_flags=(), f16: bool = False) -> str:
-    LIB = LIB_F16 if f16 else globals()["LIB"]  # noqa: N806
+    lib = LIB_F16 if f16 else LIB
     if f16:
         extra_flags = tuple(extra_flags) + ("-DHIERTCN_F16=1",)
-    ablation = False   # (the ablation library is a target of its own: build_ablation)
-    # objects live in a directory keyed on the flag set, and the library remembers which flag set it was linked from:
-    # an ablation build can never leave objects (or a library) behind that a later plain build would ship as fresh
+    # flags of the caller's have an object directory of their own, and the library remembers which flags it was linked from: an
+    # experiment can never leave objects (or a library) behind that a later plain build would ship as fresh
     import hashlib
-    user_flags = [f for f in extra_flags if f not in ("-DHIERTCN_F16=1", "-DHIERTCN_ABLATION=1")]
-    OBJ = os.path.join(HERE, "build", *(["ablation"] if ablation else []), *(["f16"] if f16 else []),  # noqa: N806
-                       *(["x" + hashlib.sha1(" ".join(user_flags).encode()).hexdigest()[:8]] if user_flags else []))
+    user_flags = [f for f in extra_flags if f != "-DHIERTCN_F16=1"]
+    obj_dir = os.path.join(OBJ, *(["f16"] if f16 else []), *(["x" + hashlib.sha1(" ".join(user_flags).encode()).hexdigest()[:8]] if user_flags else []))
     flagset = " ".join([*FLAGS, *extra_flags])
-    stamp = LIB + ".flags"
+    stamp = lib + ".flags"
     try:
         with open(stamp) as f:
             relink = f.read() != flagset
     except OSError:
         relink = True
-    os.makedirs(OBJ, exist_ok=True)
-    hipcc = _hipcc()
-    headers = _headers()
-    jobs = []
-    for src in SOURCES:
-        s = os.path.join(CSRC, src)
-        o = os.path.join(OBJ, src.replace(".hip", ".o"))
-        if force or _stale(o, [s] + headers + _ops_headers(src)):
-            jobs.append((s, o))
-
-    def cc(job):
-        s, o = job
-        # score.hip: logits are finite or -inf by construction; without NaN-honouring fmaxf needs no
-        # canonicalising v_max on MFMA results (cdna_hip_programming.md, attention 'Pitfalls')
-        per_file = ["-fno-honor-nans"] if s.endswith(NO_NAN_SOURCES) else []
-        cmd = [hipcc, *FLAGS, *per_file, *extra_flags, "-c", s, "-o", o]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("hipcc failed: %s\n%s\n%s" % (" ".join(cmd), r.stdout, r.stderr))
-        if verbose and r.stderr.strip():
-            print(r.stderr, file=sys.stderr)
-        return o
-
-    if jobs:
-        with ThreadPoolExecutor(max_workers=min(6, len(jobs))) as ex:
-            list(ex.map(cc, jobs))
-    objs = [os.path.join(OBJ, s.replace(".hip", ".o")) for s in SOURCES]
-    if force or jobs or relink or _stale(LIB, objs):
-        # nothing but the HIP runtime: every kernel of the library, the plain GEMMs of the backward pass included (csrc/gemm.hip), is its own
-        cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("link failed: %s\n%s" % (r.stdout, r.stderr))
+    objs, built = _compile(SOURCES, obj_dir, extra_flags, force, verbose)
+    if force or built or relink or _stale(lib, objs):
+        _link(lib, objs)
         with open(stamp, "w") as f:
             f.write(flagset)
-    return LIB
+    return lib
 
 
 if __name__ == "__main__":
