@@ -11,7 +11,8 @@
 // those of the tiles before it in its group of 16 to the state before the group, and the last of a group publishes the state behind it.  The order of
 // all that is the order of time, whoever waits for whom, so results do not depend on timing.  A word (A, S) is its own flag: 64 bits, written by one store that
 // goes past the L2s, all ones until then (a NaN is stored as the canonical one, so that no result looks like that).  A workgroup takes the tile of its TICKET, drawn
-// when it starts, and waits for lower tickets only: those run, and the lowest waits for nobody, so every wait ends, however workgroups are dispatched.
+// when it starts, and waits for lower tickets only: those run, and the lowest waits for nobody, so every wait ends, however workgroups are dispatched.  Should a
+// word never come all the same (a workspace that two calls use at once), its waits give up after some seconds: what could not be learnt is NaN and the launch ends.
 //
 // The backward pass is the same recurrence the other way round, lambda_t = dout_t + a_{t+1} lambda_{t+1}: with r_t = a_t lambda_t a run maps r -> A r + Q
 // with the same A.  States are not read back from the rounded output: the forward pass leaves the fp32 state before every segment in `record`, 1/16 of
@@ -25,6 +26,10 @@
 // A reset has to cut a state that is NaN or infinite (0 * NaN = NaN), and nothing else may: with a mask, A is exactly 0 only where a reset lies in the run
 // (the product of the gates alone is kept from underflowing to 0), and a map with A = 0 ignores what it is applied to.  Without one maps are plain fma's.
 #include "ops.h"
+
+#ifdef HIERTCN_TEST_HOOKS
+#include <stdlib.h>
+#endif
 
 namespace {
 
@@ -41,7 +46,8 @@ struct GlrP {
   uint64_t* map;                 // [ntile][B][D]: the tiles' maps
   uint64_t* behind;              // [ntile / GROUP][B][D]: the state behind a group, in the low half
   float* state0;                 // [B][D]: the state before the first tile (state_out may be state_in)
-  unsigned* ticket;
+  unsigned* ticket;              // and, behind it, whether a wait has given up
+  unsigned grid, polls;          // workgroups; looks of a wait
 };
 constexpr int GROUP = 16;        // tiles of a group
 
@@ -210,6 +216,11 @@ __device__ __forceinline__ void tile_scan(float2* lds, const Place<VEC>& at, con
   fold_waves<VEC, CUT, REV>(lds, at, carry, h);
 }
 
+#ifdef HIERTCN_TEST_HOOKS       // the test of the waits' bound: a launch whose words never come (GlrP's polls from the environment).  In no shipped library.
+#define GLR_PUBLISH (p.polls == OPS_POLLS)
+#else
+#define GLR_PUBLISH true
+#endif
 // ---- CHAIN ------------------------------------------------------------------------------------------------------------------------------------------
 // What a chained workgroup keeps in LDS: the maps of its waves, those of the tiles before it in its group, the state before the group, the ticket.
 template <int VEC>
@@ -243,21 +254,21 @@ __device__ __forceinline__ void chain_scan(const GlrP& p, const ChainLds<VEC>& l
     for (int q = 0; q < at.nw; q++)
 #pragma unroll
       for (int i = 0; i < VEC; i++) tA[i] = map_a<CUT>(tA[i], lds.waves[(q * VEC + i) * 64 + lane].x);
-    if (at.chan && place + 1 < GROUP)
+    if (GLR_PUBLISH && at.chan && place + 1 < GROUP)
 #pragma unroll
       for (int i = 0; i < VEC; i++) ops_publish(p.map + (int64_t)at.tile * plane + row + at.off + i, ops_word(tS[i], tA[i]));
   }
   for (int q = at.w; q < place; q += at.nw)
 #pragma unroll
     for (int i = 0; i < VEC; i++) {
-      const uint64_t v = ops_await(p.map + (int64_t)(group * GROUP + q) * plane + row + at.off + i);
+      const uint64_t v = ops_await(p.map + (int64_t)(group * GROUP + q) * plane + row + at.off + i, p.ticket + 1, p.polls);
       lds.tiles[(q * VEC + i) * 64 + lane] = make_float2(ops_high(v), ops_low(v));
     }
   if (at.w == at.nw - 1) {
     float f[VEC];
     if (group == 0) get_state<VEC>(p.state0, row, at, f);
 #pragma unroll
-    for (int i = 0; i < VEC; i++) lds.first[i * 64 + lane] = group == 0 ? f[i] : ops_low(ops_await(p.behind + (int64_t)(group - 1) * plane + row + at.off + i));
+    for (int i = 0; i < VEC; i++) lds.first[i * 64 + lane] = group == 0 ? f[i] : ops_low(ops_await(p.behind + (int64_t)(group - 1) * plane + row + at.off + i, p.ticket + 1, p.polls));
   }
   __syncthreads();
 #pragma unroll
@@ -274,7 +285,7 @@ __device__ __forceinline__ void chain_scan(const GlrP& p, const ChainLds<VEC>& l
 #pragma unroll
         for (int i = 0; i < VEC; i++) carry[i] = map_s<CUT>(m[k][i].x, carry[i], m[k][i].y);
   }
-  if (at.w == 0 && at.chan && place + 1 == GROUP && at.tile + 1 < p.ntile)
+  if (GLR_PUBLISH && at.w == 0 && at.chan && place + 1 == GROUP && at.tile + 1 < p.ntile)
 #pragma unroll
     for (int i = 0; i < VEC; i++) ops_publish(p.behind + (int64_t)group * plane + row + at.off + i, ops_word(map_s<CUT>(tA[i], carry[i], tS[i]), 0.f));
   fold_waves<VEC, CUT, REV>(lds.waves, at, carry, h);
@@ -282,7 +293,7 @@ __device__ __forceinline__ void chain_scan(const GlrP& p, const ChainLds<VEC>& l
 // clears what a chain's words start from
 __global__ __launch_bounds__(256) void k_chain_init(GlrP p, const float* first, int64_t words) {
   const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x, n = p.a.B * p.a.D;
-  if (i0 == 0) *p.ticket = 0;
+  if (i0 < 2) p.ticket[i0] = 0;
   for (int64_t i = i0; i < words; i += (int64_t)gridDim.x * 256) p.map[i] = OPS_NOTHING;
   for (int64_t i = i0; i < n; i += (int64_t)gridDim.x * 256) p.state0[i] = first ? first[i] : 0.f;
 }
@@ -293,7 +304,9 @@ __global__ __launch_bounds__(64 * MAXW / VEC) void k_glr(GlrP p) {
   extern __shared__ float2 lds[];          // 2 x [nw][VEC][64]; CHAIN: ChainLds
   const hiertcn_glr_t& a = p.a;
   const ChainLds<VEC> chain(lds);
-  const Place<VEC> at(p, CHAIN ? ops_ticket(p.ticket, chain.ticket) : blockIdx.x);
+  const unsigned blk = CHAIN ? ops_ticket(p.ticket, chain.ticket) : blockIdx.x;
+  if (CHAIN && blk >= p.grid) return;      // (never, but with a workspace that two calls use at once)
+  const Place<VEC> at(p, blk);
   const int64_t row = at.b * a.D + at.ch0;
   const int len = length_of(a, at.b), seg0 = CHAIN ? at.tile * at.nw : 0, seg1 = CHAIN && seg0 + at.nw < p.nseg ? seg0 + at.nw : p.nseg;
   float carry[VEC], h[VEC], u[SEG][VEC], s[SEG][VEC], A[VEC], S[VEC];
@@ -369,7 +382,9 @@ __global__ __launch_bounds__(64 * MAXW) void k_glr_bwd(GlrP p) {
   extern __shared__ float2 lds[];          // as in k_glr
   const hiertcn_glr_t& a = p.a;
   const ChainLds<VEC> chain(lds);
-  const Place<VEC> at(p, CHAIN ? ops_ticket(p.ticket, chain.ticket) : blockIdx.x);
+  const unsigned blk = CHAIN ? ops_ticket(p.ticket, chain.ticket) : blockIdx.x;
+  if (CHAIN && blk >= p.grid) return;      // (never, but with a workspace that two calls use at once)
+  const Place<VEC> at(p, blk);
   const int64_t row = at.b * a.D + at.ch0;
   const int len = length_of(a, at.b), seg0 = CHAIN ? (p.ntile - 1 - at.tile) * at.nw : 0, seg1 = CHAIN && seg0 + at.nw < p.nseg ? seg0 + at.nw : p.nseg;
   const int tiles = (seg1 - seg0 + at.nw - 1) / at.nw;
@@ -599,6 +614,11 @@ int glr(const hiertcn_glr_t* in, bool backward, hipStream_t st) {
     p.behind = p.map + q.ntile * a.B * a.D;
     p.state0 = reinterpret_cast<float*>(p.map + words_of(q, a.B, a.D));
     p.ticket = reinterpret_cast<unsigned*>(p.state0 + (a.B * a.D + 31) / 32 * 32);
+    p.grid = (unsigned)(q.ncb * a.B * q.ntile);
+    p.polls = OPS_POLLS;
+#ifdef HIERTCN_TEST_HOOKS
+    if (const char* polls = getenv("HIERTCN_GLR_TEST_POLLS")) p.polls = (unsigned)atoi(polls);
+#endif
   }
   const hipError_t launched = a.dtype == HIERTCN_FP32 ? go_vec<HIERTCN_FP32>(p, q, backward, st) : a.dtype == HIERTCN_BF16 ? go_vec<HIERTCN_BF16>(p, q, backward, st) : go_vec<HIERTCN_FP16>(p, q, backward, st);
   OPS_TRY(launched);

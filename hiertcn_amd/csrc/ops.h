@@ -113,9 +113,18 @@ __device__ __forceinline__ uint64_t ops_word(float lo, float hi) {      // (a Na
 __device__ __forceinline__ float ops_low(uint64_t v) { return __builtin_bit_cast(float, (uint32_t)v); }
 __device__ __forceinline__ float ops_high(uint64_t v) { return __builtin_bit_cast(float, (uint32_t)(v >> 32)); }
 __device__ __forceinline__ void ops_publish(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ uint64_t ops_await(const uint64_t* p) {
+// Waits for a word.  A wait that cannot end gives up after `polls` looks, or soon after another has (*gave_up is set then): the word is a pair of NaNs.
+constexpr unsigned OPS_POLLS = 1u << 22;      // some seconds; a word that is on its way takes microseconds
+__device__ __forceinline__ uint64_t ops_await(const uint64_t* p, unsigned* gave_up, unsigned polls) {
   uint64_t v;
-  while ((v = __hip_atomic_load(const_cast<uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == OPS_NOTHING) __builtin_amdgcn_s_sleep(1);
+  unsigned n = 0;
+  while ((v = __hip_atomic_load(const_cast<uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == OPS_NOTHING) {
+    if (++n > polls || (n % 64 == 0 && __hip_atomic_load(gave_up, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))) {
+      __hip_atomic_store(gave_up, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      return ops_word(__builtin_nanf(""), __builtin_nanf(""));
+    }
+    __builtin_amdgcn_s_sleep(1);
+  }
   return v;
 }
 // The ticket of a workgroup: the order in which workgroups START, whatever order they are dispatched in.  `place`: LDS.  One barrier.

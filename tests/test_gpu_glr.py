@@ -244,3 +244,16 @@ def test_offsets_behind_2_to_the_32():
     assert (h[4, T - 1] - 1).abs().max() < 1e-2 and (s[4] - 1).abs().max() < 1e-4 and (h[3, 4:1000] == 0).all() and (h[3, T - 1] == 0).all()
     tail = glr_scan(g[4:, :40], x[4:, :40], state[4:], cand_act="none")[0]
     assert torch.equal(h[4, :40], tail[0])
+
+
+def test_a_wait_that_cannot_be_met_gives_up():
+    """Long recurrences hand states from workgroup to workgroup; with words that never come (tests/tools/glr_wait_probe.py, the test-hooks build) the launch ends and
+    what could not be learnt is NaN."""
+    import os
+    import subprocess
+    import sys
+    from hiertcn_amd.build import LIB_TESTHOOKS
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, os.path.join(root, "tests", "tools", "glr_wait_probe.py")], env=dict(os.environ, HIERTCN_LIB=LIB_TESTHOOKS), capture_output=True, text=True,
+                       timeout=110)
+    assert r.returncode == 0 and "glr_wait_probe ok" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
