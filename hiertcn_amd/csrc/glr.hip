@@ -64,11 +64,14 @@ __device__ __forceinline__ void gate_of(float g, float& u, float& w) {
   u = g >= 0.f ? r : er;
   w = g >= 0.f ? er : r;
 }
-// tanh to a few ulp: the odd series where (1 - e^-2x) / (1 + e^-2x) would cancel
-__device__ __forceinline__ float tanh_of(float x) {
+// tanh to a few ulp: the odd series where (1 - e^-2x) / (1 + e^-2x) would cancel; and its slope 4 e^-2x / (1 + e^-2x)^2 (1 - tanh^2, formed from a rounded tanh, is
+// all error from |x| = 8 on)
+__device__ __forceinline__ float tanh_of(float x, float& slope) {
   const float a = fabsf(x), x2 = x * x;
   const float e = ops_exp(-2.f * a);
-  const float big = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x);
+  const float r = __builtin_amdgcn_rcpf(1.f + e);
+  const float big = copysignf((1.f - e) * r, x);
+  slope = 4.f * e * r * r;
   float s = fmaf(x2, -8.863235530e-3f, 2.186948854e-2f);     // x - x^3/3 + 2x^5/15 - 17x^7/315 + 62x^9/2835 - 1382x^11/155925
   s = fmaf(x2, s, -5.396825397e-2f);
   s = fmaf(x2, s, 1.333333333e-1f);
@@ -333,7 +336,8 @@ __global__ __launch_bounds__(64 * MAXW / VEC) void k_glr(GlrP p) {
         for (int i = 0; i < VEC; i++) {
           float w;
           gate_of(g4[i], u[j][i], w);
-          s[j][i] = w * (TANH ? tanh_of(c4[i]) : c4[i]);
+          float slope;
+          s[j][i] = w * (TANH ? tanh_of(c4[i], slope) : c4[i]);
         }
       }
       if (n < SEG)                         // dead steps: the identity
@@ -414,13 +418,13 @@ __global__ __launch_bounds__(64 * MAXW) void k_glr_bwd(GlrP p) {
         ops_cvt<DT, VEC>(rd[j], d[j]);
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
-          float w;
+          float w, slope = 1.f;
           gate_of(g4[i], u[j][i], w);
-          const float c = TANH ? tanh_of(c4[i]) : c4[i];
+          const float c = TANH ? tanh_of(c4[i], slope) : c4[i];
           const float hp = held<CUT>(h[i], keep, j);
           h[i] = fmaf(u[j][i], hp, w * c);
           fg[j][i] = (hp - c) * (u[j][i] * w);
-          fx[j][i] = TANH ? w * fmaf(-c, c, 1.f) : w;
+          fx[j][i] = w * slope;
         }
       }
       if (n < SEG)                         // dead steps: the identity, no gradient

@@ -49,7 +49,10 @@ def glr(gate, cand, state=None, mask=None, lengths=None, act="tanh", dh=None, ds
     d = np.asarray(dh, np.float64)
     r = np.zeros((B, D)) if dstate_out is None else np.asarray(dstate_out, np.float64).copy()
     er, rm = np.zeros((B, D)), np.abs(r)
-    slope = 1 - c * c if act == "tanh" else np.ones_like(c)
+    # 1 - tanh^2 = 4 e / (1 + e)^2 with e = exp(-2 |x|), whose exponential is within 2 |x| + 3 half steps; the reciprocal, taken twice, 1 + e and the products: 9 more
+    q = np.exp(-2 * np.abs(x))
+    slope = 4 * q / (1 + q) ** 2 if act == "tanh" else np.ones_like(c)
+    es = (2 * np.abs(x) + 12) * EPS if act == "tanh" else np.zeros_like(c)
     dg, dx, dg_err, dx_err = (np.zeros((B, T, D)) for _ in range(4))
     for t in range(T - 1, -1, -1):
         k, on = keep[:, t, None], (t < lens)[:, None]
@@ -60,7 +63,7 @@ def glr(gate, cand, state=None, mask=None, lengths=None, act="tanh", dh=None, ds
         dg[:, t] = np.where(on, lam * gap * uw, 0.0)
         dx[:, t] = np.where(on, lam * w[:, t] * slope[:, t], 0.0)
         dg_err[:, t] = np.where(on, el * np.abs(gap) * uw + np.abs(lam) * uw * (prev_err[:, t] + ec[:, t] + EPS * np.abs(gap)) + (2 * EPS_GATE + 4 * EPS) * np.abs(dg[:, t]), 0.0)
-        dx_err[:, t] = np.where(on, el * w[:, t] * slope[:, t] + np.abs(lam) * w[:, t] * (2 * np.abs(c[:, t]) * ec[:, t] + EPS) + (EPS_GATE + 4 * EPS) * np.abs(dx[:, t]), 0.0)
+        dx_err[:, t] = np.where(on, el * w[:, t] * slope[:, t] + (es[:, t] + EPS_GATE + 4 * EPS) * np.abs(dx[:, t]), 0.0)
         new = np.where(k, u[:, t] * lam, 0.0)
         err = np.where(k, u[:, t] * (el + (EPS_GATE + 2 * EPS) * lm), 0.0)
         r, er, rm = np.where(on, new, r), np.where(on, err, er), np.where(on, np.where(k, u[:, t] * lm, 0.0), rm)

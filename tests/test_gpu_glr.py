@@ -257,3 +257,13 @@ def test_a_wait_that_cannot_be_met_gives_up():
     r = subprocess.run([sys.executable, os.path.join(root, "tests", "tools", "glr_wait_probe.py")], env=dict(os.environ, HIERTCN_LIB=LIB_TESTHOOKS), capture_output=True, text=True,
                        timeout=110)
     assert r.returncode == 0 and "glr_wait_probe ok" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(3, 50, 64), (1, 3000, 64), (700, 6, 128)], ids=str)
+def test_gradients_of_saturated_candidates(shape, dtype):
+    """|cand| of 5 to 20: the slope of tanh there is 2e-4 to 2e-17 and the gradient as exact, relative to itself, as anywhere."""
+    g, x, dh, state, ds, mask, lengths = inputs(*shape, dtype, seed=91)
+    size = 5 + 15 * torch.rand(x.shape, generator=torch.Generator().manual_seed(4))
+    x = torch.where(torch.rand(x.shape, generator=torch.Generator().manual_seed(5)) < 0.5, -size, size).to(dtype).cuda()
+    check(g, x, dh, state, ds, mask, lengths, "tanh")
