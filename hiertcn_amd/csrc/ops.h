@@ -133,5 +133,10 @@ __device__ __forceinline__ unsigned ops_ticket(unsigned* counter, unsigned* plac
   __syncthreads();
   return (unsigned)__builtin_amdgcn_readfirstlane((int)*place);
 }
-// 2^x through v_exp_f32 (one ulp); e^x for |x| that matter here
+// e^x for x <= 0 through v_exp_f32 (one ulp).  The product x log2 e is rounded: |x| half steps of the result, too few to matter behind a 16-bit rounding.
 __device__ __forceinline__ float ops_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+// The same to 3 half steps and |x| / 20: with t = x log2 e as rounded, e^x = 2^t e^(x - t ln 2), whose second factor is 1 + (x - t ln 2) to 2^-33.
+__device__ __forceinline__ float ops_exp_fp32(float x) {
+  const float t = x * 1.4426950408889634f, e = __builtin_amdgcn_exp2f(t);
+  return e == 0.f ? e : fmaf(e, fmaf(t, -0.6931471805599453f, x), e);      // (x may be -infinity)
+}

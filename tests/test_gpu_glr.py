@@ -267,3 +267,13 @@ def test_gradients_of_saturated_candidates(shape, dtype):
     size = 5 + 15 * torch.rand(x.shape, generator=torch.Generator().manual_seed(4))
     x = torch.where(torch.rand(x.shape, generator=torch.Generator().manual_seed(5)) < 0.5, -size, size).to(dtype).cuda()
     check(g, x, dh, state, ds, mask, lengths, "tanh")
+
+
+@pytest.mark.parametrize("shape", [(3, 40, 64), (1, 2000, 64), (700, 6, 128)], ids=str)
+@pytest.mark.parametrize("size", [8, 30, 80])
+def test_gates_far_open_and_shut(size, shape):
+    """fp32 gates of up to +-80: the small one of u and 1 - u is as exact, relative to itself, as the other.  (Its exponential is within 3 half steps + 1/20 of |x|; 1 + e,
+    the reciprocal, the product: 5 more, 12 in all at |gate| = 80; the bound counts 16.)"""
+    g, x, dh, state, ds, mask, lengths = inputs(*shape, torch.float32, seed=93)
+    g = (size * (2 * torch.rand(g.shape, generator=torch.Generator().manual_seed(size)) - 1)).cuda()
+    check(g, x, dh, state, ds, mask, lengths, "tanh")
