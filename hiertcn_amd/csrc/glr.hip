@@ -23,8 +23,9 @@
 // instructions) at 2 x 65536 x 512 bf16 chained, 93 / 137 (4.2 / 4.8 TB/s) at 128 x 2000 x 128 fp32; a copy of many GB runs at 4.8.  A single step of 32 x 256: 4.8 us,
 // a launch.  Fetching the next tile before the fold of this one costs registers and waves: 114 -> 155 chained, nothing gained elsewhere.
 //
-// A reset has to cut a state that is NaN or infinite (0 * NaN = NaN), and nothing else may: with a mask, A is exactly 0 only where a reset lies in the run
-// (the product of the gates alone is kept from underflowing to 0), and a map with A = 0 ignores what it is applied to.  Without one maps are plain fma's.
+// A reset has to cut a state that is NaN or infinite (0 * NaN = NaN), and nothing else may: A is exactly 0 only where a reset lies in the run, and a map with A = 0
+// ignores what it is applied to.  The product of the gates alone is kept from underflowing to 0: an infinite state stays infinite however many gates are all but
+// shut (0 * inf = NaN).  Without a mask maps are plain fma's.
 #include "ops.h"
 
 #ifdef HIERTCN_TEST_HOOKS
@@ -53,7 +54,7 @@ constexpr int GROUP = 16;        // tiles of a group
 
 // maps: composition and application.  CUT: A = 0 marks a reset
 template <bool CUT>
-__device__ __forceinline__ float map_a(float A1, float A2) { return !CUT ? A1 * A2 : A1 == 0.f || A2 == 0.f ? 0.f : fmaxf(A1 * A2, TINY); }
+__device__ __forceinline__ float map_a(float A1, float A2) { return !CUT ? fmaxf(A1 * A2, TINY) : A1 == 0.f || A2 == 0.f ? 0.f : fmaxf(A1 * A2, TINY); }
 template <bool CUT>
 __device__ __forceinline__ float map_s(float A2, float S1, float S2) { return CUT && A2 == 0.f ? S2 : fmaf(A2, S1, S2); }
 
@@ -173,9 +174,8 @@ __device__ __forceinline__ void store_rows(const char* q, int64_t st, const Plac
 // the product of a segment's gates as the A of its map
 template <int VEC, bool CUT>
 __device__ __forceinline__ void close_map(uint32_t keep, float (&A)[VEC]) {
-  if (CUT)
 #pragma unroll
-    for (int i = 0; i < VEC; i++) A[i] = keep == 0xffffffffu ? (A[i] == A[i] ? fmaxf(A[i], TINY) : A[i]) : 0.f;
+  for (int i = 0; i < VEC; i++) A[i] = !CUT || keep == 0xffffffffu ? (A[i] < TINY ? TINY : A[i]) : 0.f;      // (a NaN stays)
 }
 
 // The state before (REV: behind) every wave's segment, given `carry` before the tile; `carry` behind it.  One barrier; `lds` alternates between two buffers, so

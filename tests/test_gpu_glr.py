@@ -277,3 +277,27 @@ def test_gates_far_open_and_shut(size, shape):
     g, x, dh, state, ds, mask, lengths = inputs(*shape, torch.float32, seed=93)
     g = (size * (2 * torch.rand(g.shape, generator=torch.Generator().manual_seed(size)) - 1)).cuda()
     check(g, x, dh, state, ds, mask, lengths, "tanh")
+
+
+@pytest.mark.parametrize("resets", [False, True])
+@pytest.mark.parametrize("T", [12, 300, 20000])
+def test_an_infinite_state_stays_infinite(T, resets):
+    """Gates of 1e-13 all along (16 of them multiply to less than fp32 holds): h = u inf + (1 - u) c is infinite at every step, forward and backward, until a reset."""
+    from hiertcn_amd.glr import glr_scan, glr_scan_backward
+    B, D = 2, 64
+    g, x, dh, state, ds, _, _ = inputs(B, T, D, torch.float32, seed=95, ragged=False, resets=False)
+    g = torch.full_like(g, -30.0)
+    mask = torch.ones(B, T, device="cuda") if resets else None
+    if resets:
+        mask[1, T - 3] = 0
+    bad, dbad = state.clone(), ds.clone()
+    bad[:, ::2], dbad[:, 1::2] = float("inf"), float("-inf")
+    h, s, rec = glr_scan(g, x, bad, mask=mask, want_record=True)
+    rows = h[1, :T - 3] if resets else h[1]
+    assert torch.isposinf(h[0, :, ::2]).all() and torch.isposinf(s[0, ::2]).all() and torch.isposinf(rows[:, ::2]).all() and torch.isfinite(h[:, :, 1::2]).all()
+    if resets:
+        assert torch.isfinite(h[1, T - 3:]).all() and torch.isfinite(s[1]).all()
+    _, dx, d0 = glr_scan_backward(g, x, dh, glr_scan(g, x, state, mask=mask, want_record=True)[2], mask=mask, dstate_out=dbad)
+    assert torch.isneginf(dx[0, :, 1::2]).all() and torch.isneginf(d0[0, 1::2]).all() and torch.isfinite(dx[:, :, ::2]).all()
+    if resets:
+        assert torch.isneginf(dx[1, T - 3:, 1::2]).all() and torch.isfinite(dx[1, :T - 3]).all() and torch.isfinite(d0[1]).all()
