@@ -340,8 +340,10 @@ __device__ __forceinline__ Answer answer_of(const hiertcn_policy_t& q, int64_t T
   if (q.ref_logp) {
     const double gap = q.ref_logp[r] - lp, e = expm1(gap);
     o.kl = e == INFINITY ? e : e - gap;
-    o.loss += q.kl_coef * o.kl;
-    o.c += q.kl_coef * -e;
+    if (q.kl_coef != 0.f) {             // (an infinite kl that is only looked at leaves the loss alone)
+      o.loss += q.kl_coef * o.kl;
+      o.c += q.kl_coef * -e;
+    }
   }
   o.loss *= weight;
   o.kl *= weight;

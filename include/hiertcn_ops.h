@@ -105,9 +105,10 @@ int hiertcn_preference_loss(const hiertcn_rows_t* r, const hiertcn_preference_t*
 
 /* Clipped policy loss with a penalty on the distance from a reference, per answer:
  *   ratio = exp(logp - old), l = -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef k,  k = exp(ref - logp) - (ref - logp) - 1
- * (A = 0: the first term is 0).  loss [1] = mean over every sequence's answers, then over the sequences that have any (mean 0: the lane mean of
- * model.py:111-117), or over all answers (mean 1); 0 where there is none.  kl [1], clipped [1]: the same means of k and of [the clamp is the
- * smaller branch].  The losses take logp before it is rounded to fp32 (a ratio to an old that is this very logp is 1 to within that rounding).
+ * (A = 0: the first term is 0.  kl_coef = 0: so is the penalty, though kl is reported, whatever it is: inf where an answer's logit is -inf).
+ * loss [1] = mean over every sequence's answers, then over the sequences that have any (mean 0: the lane mean of model.py:111-117), or over all answers
+ * (mean 1); 0 where there is none.  kl [1], clipped [1]: the same means of k and of [the clamp is the smaller branch].  The losses take logp before it
+ * is rounded to fp32 (a ratio to an old that is this very logp is 1 to within that rounding).
  * old, ref [n][T]; advantage [n][T] with element strides (adv_sn, adv_st), 0 = broadcast. */
 typedef struct {
   int32_t mean, reserved;

@@ -295,3 +295,30 @@ def test_a_pair_of_very_long_sequences():
     want = torch.where(ok[..., None], want, torch.zeros(()).double())
     got = out["dlogits"].double().cpu()
     assert (got[~ok] == 0).all() and ((got - want)[ok].abs() <= 1e-3 * abs(c) + 1000.0 * beta ** 2 / 4 * 2 * bound).all()
+
+
+@pytest.mark.parametrize("A", [1.5, -1.5])
+def test_an_impossible_answer_under_the_policy_loss(A):
+    """The logit of an answer is -inf: ratio 0, so the clipped term is 0 (A > 0) or decided by the clamp (A < 0), and its gradient 0.  A reference that is only
+    monitored (kl_coef = 0) leaves loss and gradient as they are without it, whether it masks the item too or not; with a coefficient the penalty is infinite."""
+    from hiertcn_amd.sequence_loss import policy_loss
+    z, ids, _ = make(2, 3, 60, torch.float32, seed=29)
+    ids[:] = 7
+    z[0, 1, 7] = float("-inf")
+    old = torch.full((2, 3), -4.0, device="cuda")
+    adv = torch.full((2,), A, device="cuda")
+    plain = policy_loss(z, ids, old, adv)
+    assert plain["logp"][0, 1] == float("-inf") and torch.isfinite(plain["loss"]) and (plain["dlogits"][0, 1] == 0).all() and torch.isfinite(plain["dlogits"]).all()
+    lp = SO.rows(n64(z), ids.cpu().numpy())["logp"]
+    ratio = np.exp(lp + 4.0)
+    term = -np.minimum(ratio * A, np.clip(ratio, 1 - float(np.float32(0.2)), 1 + float(np.float32(0.2))) * A)
+    assert abs(float(plain["loss"]) - term.mean(1).mean()) < 1e-5
+    for there in (-3.0, float("-inf")):
+        ref = torch.full((2, 3), -3.5, device="cuda")
+        ref[0, 1] = there
+        out = policy_loss(z, ids, old, adv, ref_logp=ref)
+        assert torch.equal(out["loss"], plain["loss"]) and torch.equal(out["dlogits"], plain["dlogits"]) and torch.equal(out["clipped"], plain["clipped"])
+        assert not torch.isfinite(out["kl"])
+    ref[0, 1] = -3.0
+    out = policy_loss(z, ids, old, adv, ref_logp=ref, kl_coef=0.1)
+    assert torch.isposinf(out["loss"]) and torch.isposinf(out["kl"]) and torch.isfinite(out["dlogits"][0, 0]).all() and torch.isfinite(out["dlogits"][1]).all()
