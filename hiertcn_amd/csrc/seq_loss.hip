@@ -46,11 +46,15 @@ __device__ __forceinline__ bool answered(const hiertcn_rows_t& a, int64_t r, int
   return y > 0 && y < a.V;
 }
 
+// exp of what is at most 0.  fp32 logits: to 3 half steps wherever it lies; 16-bit ones: |x| half steps of fp32 more, behind a rounding of 2^13 or more of them
+template <int DT>
+__device__ __forceinline__ float exp_of(float x) { return DT == HIERTCN_FP32 ? ops_exp_fp32(x) : ops_exp(x); }
+
 // (m, s) of two runs as one.  m = -inf: nothing in it (s is 0, or NaN and stays NaN).
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2), ref = ref_of(top);
-  s = s * ops_exp(m - ref) + s2 * ops_exp(m2 - ref);
+  s = s * ops_exp_fp32(m - ref) + s2 * ops_exp_fp32(m2 - ref);
   m = top;
 }
 __device__ __forceinline__ void wave_join(float& m, float& s) {
@@ -114,12 +118,12 @@ __device__ __forceinline__ void fold(const typename OpsRaw<DT, VEC>::type (&x)[U
     }
   }
   const float ref = ref_of(top);
-  s *= ops_exp(m - ref);
+  s *= exp_of<DT>(m - ref);
   m = top;
 #pragma unroll
   for (int u = 0; u < U; u++)
 #pragma unroll
-    for (int i = 0; i < VEC; i++) s += ops_exp(z[u][i] - ref);
+    for (int i = 0; i < VEC; i++) s += exp_of<DT>(z[u][i] - ref);
 }
 
 // answers per sequence, and this workgroup's share of their totals: a thread a sequence where sequences are short, else a wave
@@ -183,7 +187,7 @@ __global__ __launch_bounds__(NT) void k_part(RowsP p) {
   if (e >= 0) {
     float z[1];
     ops_ld<DT, 1>(row, e, z);
-    join(m, s, z[0], z[0] == -INFINITY ? 0.f : ops_exp(z[0] - z[0]));
+    join(m, s, z[0], z[0] == -INFINITY ? 0.f : 1.f + (z[0] - z[0]));
   }
   wave_join(m, s);
   if constexpr (TPR == NT) {
@@ -395,7 +399,7 @@ __device__ __forceinline__ void gradient_of(const typename OpsRaw<DT, VEC>::type
   float z[VEC];
   ops_cvt<DT, VEC>(x, z);
 #pragma unroll
-  for (int i = 0; i < VEC; i++) z[i] = g * ops_exp(z[i] - ref);
+  for (int i = 0; i < VEC; i++) z[i] = g * exp_of<DT>(z[i] - ref);
   if (y >= at && y - at < VEC)
 #pragma unroll
     for (int i = 0; i < VEC; i++) z[i] += i == y - at ? c : 0.f;
@@ -450,7 +454,7 @@ __global__ __launch_bounds__(NT) void k_dlogits(RowsP p, Sums q) {
   if (e >= 0) {
     float z[1];
     ops_ld<DT, 1>(row, e, z);
-    z[0] = g * ops_exp(z[0] - ref);
+    z[0] = g * exp_of<DT>(z[0] - ref);
     if (e == y) z[0] += c;
     ops_st<DT, 1>(out, e, z);
   }

@@ -322,3 +322,24 @@ def test_an_impossible_answer_under_the_policy_loss(A):
     ref[0, 1] = -3.0
     out = policy_loss(z, ids, old, adv, ref_logp=ref, kl_coef=0.1)
     assert torch.isposinf(out["loss"]) and torch.isposinf(out["kl"]) and torch.isfinite(out["dlogits"][0, 0]).all() and torch.isfinite(out["dlogits"][1]).all()
+
+
+@pytest.mark.parametrize("layout", ["plain", "shifted"])
+@pytest.mark.parametrize("V", [61, 4003])
+def test_the_gradient_of_far_logits(V, layout):
+    """fp32 logits up to 80 below their row's largest (multiples of 1/1024: differences are exact).  dz_j / dz_max = exp(z_j - z_max) for unanswered j, whatever sum and
+    coefficient are: the exponential is within 3 half steps + 1/20 of |x|, dz_j and dz_max one rounding each."""
+    from hiertcn_amd.sequence_loss import preference_loss
+    rng = np.random.default_rng(V)
+    z = torch.tensor(rng.integers(-80 * 1024, 0, (2, 2, V)) / 1024, dtype=torch.float32)
+    z[..., 5] = 0.0
+    ids = torch.full((2, 2), 9, dtype=torch.int32).cuda()
+    if layout == "shifted":
+        buf = torch.empty(z.numel() + 3, device="cuda")
+        buf[3:] = z.reshape(-1).cuda()
+        z = buf[3:].view(2, 2, V)
+    d = n64(preference_loss(z.cuda(), ids, torch.zeros(2, device="cuda"), beta=0.5, grad_scale=2.0 ** 20)["dlogits"])
+    x = n64(z)
+    others = np.arange(V) != 9
+    ratio, want = (d / d[..., 5:6])[..., others], np.exp(x)[..., others]
+    assert (np.abs(ratio - want) <= (6 + np.abs(x[..., others]) / 20) * HALF[torch.float32] * want).all()
