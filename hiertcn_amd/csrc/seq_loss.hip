@@ -20,6 +20,7 @@ namespace {
 
 constexpr int NT = 256;                 // threads of a workgroup
 constexpr int MAX_PARTS = 64;           // a wave joins a row's parts, one to a lane
+constexpr int64_t MAX_V = 0x7fffffff - 4096;      // elements and vectors of a row are ints, and a thread's next ones are at most 4 NT behind the last
 
 // how a row is split over workgroups
 struct Cut {
@@ -62,7 +63,7 @@ __device__ __forceinline__ void wave_join(float& m, float& s) {
   for (int d = 32; d; d >>= 1) join(m, s, __shfl_xor(m, d), __shfl_xor(s, d));
 }
 
-// the part of a row as [head] vectors [tail]: head elements up to the first address that a vector may be loaded from.  (V < 2^31: ints.)
+// the part of a row as [head] vectors [tail]: head elements up to the first address that a vector may be loaded from.  (V <= MAX_V: ints.)
 template <int DT, int VEC>
 struct Span {
   int head, v0, v1;                     // v0 .. v1: this part's vectors; element of vector v: head + v * VEC
@@ -512,7 +513,7 @@ int prepare(const hiertcn_rows_t* in, bool grad, RowsP& p, int& vec) {
   hiertcn_rows_t& a = p.a;
   if (!grad) a.dlogits = nullptr;
   if (a.n < 1 || a.T < 1 || a.V < 1) return ops_fail(HIERTCN_ERR_INVALID, "n, T and V are at least 1 (%lld, %lld, %lld)", (long long)a.n, (long long)a.T, (long long)a.V);
-  if (a.n > (1ll << 31) || a.T > (1ll << 31) || a.n * a.T > (1ll << 31) || a.V > 0x7fffffff) return ops_fail(HIERTCN_ERR_INVALID, "n * T is at most 2^31, V below 2^31");
+  if (a.n > (1ll << 31) || a.T > (1ll << 31) || a.n * a.T > (1ll << 31) || a.V > MAX_V) return ops_fail(HIERTCN_ERR_INVALID, "n * T is at most 2^31, V at most 2^31 - 4097");
   if (!ops_dtype_ok(a.dtype)) return ops_fail(HIERTCN_ERR_INVALID, "dtype %d: 0 fp32, 1 bf16, 2 fp16", a.dtype);
   if (!a.logits || !a.ids || !a.logp) return ops_fail(HIERTCN_ERR_INVALID, "null logits, ids or logp");
   p.R = a.n * a.T;
@@ -584,7 +585,7 @@ int finish(const RowsP& p, int vec, const Sums& s, hipStream_t st) {
 extern "C" {
 
 size_t hiertcn_rows_workspace_bytes(int64_t n, int64_t T, int64_t V) {
-  return n < 1 || T < 1 || V < 1 || n > (1ll << 31) || T > (1ll << 31) || n * T > (1ll << 31) || V > 0x7fffffff ? 0 : workspace_of(n, T, V, nullptr);
+  return n < 1 || T < 1 || V < 1 || n > (1ll << 31) || T > (1ll << 31) || n * T > (1ll << 31) || V > MAX_V ? 0 : workspace_of(n, T, V, nullptr);
 }
 
 int hiertcn_sequence_logp(const hiertcn_rows_t* r, void* stream) {

@@ -70,7 +70,7 @@ int hiertcn_glr_backward(const hiertcn_glr_t* a, void* stream);
 /* ---- losses on the log-probabilities of answers, with their gradients ----------------------------------------------------------------------
  * logits [n * T][V] of n sequences (row stride ld >= V elements), ids [n * T]: the item answered with at every step, 0 = none (padding).  A row whose id
  * lies outside 1 .. V-1 is not read, has log-probability 0 and gradient 0; so is a row of nothing but -inf (no distribution is left).  Column 0 takes part in
- * the soft-max, as in model_tcn.py:41.   logp = z[id] - log sum_j exp z_j
+ * the soft-max, as in model_tcn.py:41.   logp = z[id] - log sum_j exp z_j.   V is at most 2^31 - 4097.
  * dlogits (rows of stride dld, the logits' type) may be the logits' own buffer (ptr and stride equal): it is overwritten row by row. */
 typedef struct {
   int64_t n, T, V;

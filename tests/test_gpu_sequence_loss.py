@@ -343,3 +343,25 @@ def test_the_gradient_of_far_logits(V, layout):
     others = np.arange(V) != 9
     ratio, want = (d / d[..., 5:6])[..., others], np.exp(x)[..., others]
     assert (np.abs(ratio - want) <= (6 + np.abs(x[..., others]) / 20) * HALF[torch.float32] * want).all()
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+def test_the_longest_row(aligned):
+    """V = 2^31 - 4097, 16 bytes at a time and (gradient rows of another alignment) one element at a time.  2^31 ones are summed exactly up to 2^24 a thread and joined."""
+    from hiertcn_amd.sequence_loss import policy_loss
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("16 GiB of device memory")
+    V = 2 ** 31 - 4097
+    z = torch.zeros(1, 1, V, dtype=torch.bfloat16, device="cuda")
+    z[0, 0, V - 1] = 20.0
+    buf = torch.full((V + 1,), 3.0, dtype=torch.bfloat16, device="cuda")
+    d = (buf[:V] if aligned else buf[1:]).view(1, 1, V)
+    p = np.exp(20.0) / (V - 1 + np.exp(20.0))
+    ids = torch.full((1, 1), V - 1, dtype=torch.int32, device="cuda")
+    out = policy_loss(z, ids, torch.full((1, 1), float(np.log(p)), device="cuda"), torch.ones(1, device="cuda"), grad_scale=2.0 ** 20, dlogits=d)
+    assert abs(float(out["logp"]) - np.log(p)) < 1e-5 and abs(float(out["loss"]) + 1) < 1e-5
+    each = 2.0 ** 20 * p / np.exp(20.0)
+    assert abs(float(d[0, 0, V - 1]) + 2.0 ** 20 * (1 - p)) <= 2.0 ** 20 * (1 - p) * (2.0 ** -8 + 1e-5)
+    head = d[0, 0, :V - 1]
+    assert (head == head[0]).all() and abs(float(head[0]) - each) <= each * (2.0 ** -8 + 1e-5)
+    assert float(buf[V] if aligned else buf[0]) == 3.0

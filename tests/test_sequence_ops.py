@@ -342,3 +342,18 @@ def test_optimizer_tensors_share_no_memory():
     for lists in ([("params", [buf, buf])], [("params", [buf[:5]]), ("copies", [buf[4:]])], [("params", [buf[2:4], buf[9:], buf[:3]])]):
         with pytest.raises(HierTCNError, match="overlap"):
             _apart(lists)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("back", [1, 4096])
+def test_losses_refuse_rows_that_their_indices_cannot_walk(lib, dtype, back):
+    """A thread's last step goes up to 1024 vectors behind the row: V close to 2^31 would take its index over the edge (whole rows of workspaces and addresses here)."""
+    V = 2 ** 31 - back
+    assert lib.hiertcn_rows_workspace_bytes(2, 1, V) == 0 and lib.hiertcn_rows_workspace_bytes(2, 1, 2 ** 31 - 4097) > 0
+    at = lambda k: (1 << 44) + (k << 36)  # noqa: E731
+    r = _ops.Rows(n=2, T=1, V=V, dtype=dtype, ld=V, dld=V, grad_scale=1.0, logits=at(0), ids=at(1), logp=at(2), dlogits=at(3) + 4, workspace=at(4), workspace_bytes=1 << 30)
+    q = outputs(_ops.Preference(kind=0, beta=0.1), ("ref", "loss", "pair_loss", "margin", "seq_logp"))
+    o = outputs(_ops.Policy(clip_low=0.2, clip_high=0.2), ("old_logp", "advantage", "loss", "kl", "clipped"))
+    for call in (lambda: lib.hiertcn_sequence_logp(C.byref(r), None), lambda: lib.hiertcn_preference_loss(C.byref(r), C.byref(q), None),
+                 lambda: lib.hiertcn_policy_loss(C.byref(r), C.byref(o), None)):
+        assert call() == -1 and b"at most 2^31 - 4097" in lib.hiertcn_ops_last_error()
