@@ -12,6 +12,7 @@ from ._lib import HierTCNError
 from ._ops import need
 
 BLOCK = 256      # elements that share a scale of the 8-bit states
+_address = torch.Tensor.data_ptr
 
 
 def _apart(lists):
@@ -30,7 +31,10 @@ class AdamW:
     set_state takes them, in place of zeros of the optimizer's own.
 
     The step number is the object's (`t`), so a step cannot be captured into a graph (it would replay with the same bias corrections): it is refused
-    there, as the framework's graphs leave Adam outside."""
+    there, as the framework's graphs leave Adam outside.
+
+    A tensor that has other memory at the next step (`p.data = ...`, `set_`, `resize_`) is taken anew, with all the checks of the constructor: parameters, copies, bound
+    gradients and states of the caller's own are looked at every time.  (The memory they had is held until then.)"""
 
     def __init__(self, params: Sequence[torch.Tensor], grads: Optional[Sequence[Optional[torch.Tensor]]] = None, lr: float = 1e-3, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: Union[float, Sequence[float]] = 0.0, state_bits: int = 32,
@@ -43,7 +47,7 @@ class AdamW:
         n = len(self.params)
         self.device = _ops.on_gpu(self.params[0], "params[0]")
         for i, p in enumerate(self.params):
-            need(p, f"params[{i}]", torch.float32, self.device, p.shape if isinstance(p, torch.Tensor) else ())
+            self._master(p, i)
         copies = [None] * n if copies is None else list(copies)
         if len(copies) != n:
             raise HierTCNError(f"{n} parameters, {len(copies)} copies")
@@ -52,23 +56,24 @@ class AdamW:
         self._desc = (_ops.AdamwTensor * n)()
         self._flat_numel = [p.numel() for p in self.params]
         self._flat = [torch.Size([k]) for k in self._flat_numel]
-        for i, (p, c, d) in enumerate(zip(self.params, copies, self._desc)):
-            d.numel, d.param, d.index = p.numel(), p.data_ptr(), i
-            if c is not None:
-                if not isinstance(c, torch.Tensor) or c.dtype not in (torch.bfloat16, torch.float16):
-                    raise HierTCNError(f"copies[{i}]: a bfloat16 or float16 tensor")
-                d.copy, d.copy_dtype = need(c, f"copies[{i}]", c.dtype, self.device, p.shape).data_ptr(), _ops.DTYPE[c.dtype]
+        for i, (d, k) in enumerate(zip(self._desc, self._flat_numel)):
+            d.numel, d.index = k, i
         self.set_weight_decay(weight_decay)
+        self.grads = None
         if state is not None:
             self._take(state)
         else:
+            self._callers = False                  # whether the states are tensors of the caller's
             zeros = lambda dt, block=1: [torch.zeros(-(-p.numel() // block), dtype=dt, device=self.device) for p in self.params]  # noqa: E731
             self._attach(*((zeros(torch.float32), zeros(torch.float32), None, None) if state_bits == 32 else
                            (zeros(torch.int8), zeros(torch.uint8), zeros(torch.float32, BLOCK), zeros(torch.float32, BLOCK))))
-        self.grads = None
         if grads is not None:
             self._bind(grads)
             self.grads = list(grads)
+            self._watch()
+
+    def _master(self, p, i):
+        return need(p, f"params[{i}]", torch.float32, self.device, p.shape if isinstance(p, torch.Tensor) else ())
 
     def set_weight_decay(self, weight_decay: Union[float, Sequence[float]]):
         """One value, or one per tensor, from the next step on."""
@@ -86,11 +91,43 @@ class AdamW:
         names = (("m", m, dm, 1), ("v", v, dv, 1)) + ((("m_scale", m_scale, torch.float32, BLOCK), ("v_scale", v_scale, torch.float32, BLOCK)) if self.state_bits == 8 else ())
         found = [[need(t, f"{name}[{i}]", dt, self.device, torch.Size([-(-k // block)])).data_ptr() for i, (t, k) in enumerate(zip(ts, self._flat_numel))]
                  for name, ts, dt, block in names]
+        rows = []
+        for i, (p, c, k) in enumerate(zip(self.params, self.copies, self._flat_numel)):
+            if self._master(p, i).numel() != k:
+                raise HierTCNError(f"params[{i}]: {p.numel()} elements, the optimizer was built on {k}")
+            if c is not None and (not isinstance(c, torch.Tensor) or c.dtype not in (torch.bfloat16, torch.float16)):
+                raise HierTCNError(f"copies[{i}]: a bfloat16 or float16 tensor")
+            rows.append((p.data_ptr(), None, 0) if c is None else (p.data_ptr(), need(c, f"copies[{i}]", c.dtype, self.device, p.shape).data_ptr(), _ops.DTYPE[c.dtype]))
         _apart((("params", self.params), ("copies", self.copies), ("m", m), ("v", v), ("m_scale", m_scale), ("v_scale", v_scale)))
         for (name, _, _, _), ptrs in zip(names, found):
             for d, ptr in zip(self._desc, ptrs):
                 setattr(d, name, ptr)
+        for d, row in zip(self._desc, rows):
+            d.param, d.copy, d.copy_dtype = row
         self.m, self.v, self.m_scale, self.v_scale = m, v, m_scale, v_scale
+        self._shapes = [p.shape for p in self.params]
+        self._watch()
+
+    def _watch(self):
+        """Notes where the tensors are whose memory a program may exchange, and holds all that the descriptors name: an address that is still the same is the same memory."""
+        states = [t for ts in (self.m, self.v, self.m_scale, self.v_scale) for t in ts or ()]
+        theirs = states if self._callers else []
+        self._watched = theirs + [t for t in (*self.params, *self.copies, *(self.grads or ())) if t is not None]
+        self._watched_states = len(theirs)
+        self._at = [*map(_address, self._watched)]
+        self._held = [t.detach() for t in (*self._watched, *states)]
+
+    def _follow(self, states_only: bool = False):
+        """Takes tensors that have other memory than at the last look anew."""
+        watched, at = self._watched, self._at
+        if states_only and at is not None:
+            watched, at = watched[:self._watched_states], at[:self._watched_states]
+        if [*map(_address, watched)] != at:
+            self._attach(self.m, self.v, self.m_scale, self.v_scale)
+            if self.grads is not None:
+                at, self._at = self._at, None              # (refused gradients: not taken, and refused again)
+                self._bind(self.grads)
+                self._at = at
 
     def set_state(self, m, v, t: int, m_scale=None, v_scale=None):
         """Takes flat tensors as the states THEMSELVES (no copy): fp32 moments, or int8 / uint8 codes with their scales [ceil(numel / 256)]; t: steps taken."""
@@ -103,7 +140,12 @@ class AdamW:
         lists = [list(x) if x is not None else None for x in (*state, None, None)[:4]]
         if any(x is not None and len(x) != len(self.params) for x in lists) or None in lists[:2] or (self.state_bits == 8) != (None not in lists[2:]):
             raise HierTCNError("one m and one v per parameter, and a scale of each with 8-bit states only")
-        self._attach(*lists)
+        before, self._callers = getattr(self, "_callers", True), True
+        try:
+            self._attach(*lists)
+        except Exception:
+            self._callers = before
+            raise
 
     def state_dict(self) -> dict:
         """t, seed and the states on the host (checkpoints)."""
@@ -129,16 +171,17 @@ class AdamW:
         if len(grads) != len(self.params):
             raise HierTCNError(f"{len(self.params)} parameters, {len(grads)} gradients")
         found = []
-        for i, (p, g) in enumerate(zip(self.params, grads)):
+        for i, (shape, g) in enumerate(zip(self._shapes, grads)):
             if g is not None and (not isinstance(g, torch.Tensor) or g.dtype not in _ops.DTYPE):
                 raise HierTCNError(f"grads[{i}]: a float32, bfloat16 or float16 tensor")
-            found.append((None, 0) if g is None else (need(g, f"grads[{i}]", g.dtype, self.device, p.shape).data_ptr(), _ops.DTYPE[g.dtype]))
+            found.append((None, 0) if g is None else (need(g, f"grads[{i}]", g.dtype, self.device, shape).data_ptr(), _ops.DTYPE[g.dtype]))
         for d, (ptr, dtype) in zip(self._desc, found):
             d.grad, d.grad_dtype = ptr, dtype
 
     def step(self, grads: Optional[Sequence[Optional[torch.Tensor]]] = None, lr: Optional[float] = None, grad_scale: Union[float, torch.Tensor] = 1.0):
         """One step.  grads: this step's (default: the buffers given to the constructor); a parameter without one is left as it is.  grad_scale multiplies
         every gradient: a number, or a device float32 tensor of one element (clipping by the global norm)."""
+        self._follow()
         if grads is not None:
             self._bind(grads)
         elif self.grads is None:
@@ -168,6 +211,7 @@ class AdamW:
                         dst.copy_(src)
                 return out
             return self.m, self.v
+        self._follow(states_only=True)
         n = len(self.params)
         if out is None:
             out = tuple([torch.empty(p.numel(), dtype=torch.float32, device=self.device) for p in self.params] for _ in range(2))

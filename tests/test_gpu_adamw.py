@@ -254,3 +254,23 @@ def test_a_refused_binding_leaves_the_optimizer_as_it_was(bits):
     a.step()
     b.step()
     assert all(torch.equal(x, y) for x, y in zip(params + a.m + a.v, twin + b.m + b.v)) and not any(x.any() for x in z)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_moved(bits):
+    """p.data = other memory between steps, as loading and resharding do: the step goes there, and what held the parameter before is not written any more."""
+    from hiertcn_amd.adamw import AdamW
+    params, grads, _ = tensors([700, 300], 15)
+    twin = [p.clone() for p in params]
+    copies, tcopies = ([torch.empty_like(p, dtype=torch.bfloat16) for p in params] for _ in range(2))
+    a, b = AdamW(params, grads, copies=copies, state_bits=bits, seed=3), AdamW(twin, [g.clone() for g in grads], copies=tcopies, state_bits=bits, seed=3)
+    a.step()
+    b.step()
+    old = [p.data for p in params]
+    kept = [o.clone() for o in old]
+    for p, g, c in zip(params, grads, copies):
+        p.data, g.data, c.data = p.data.clone(), g.data.clone(), c.data.clone()
+    a.step()
+    b.step()
+    assert all(torch.equal(x, y) for x, y in zip(params + copies + list(a.m), twin + tcopies + list(b.m)))
+    assert all(torch.equal(o, k) for o, k in zip(old, kept)) and not torch.equal(params[0], kept[0])

@@ -357,3 +357,78 @@ def test_losses_refuse_rows_that_their_indices_cannot_walk(lib, dtype, back):
     for call in (lambda: lib.hiertcn_sequence_logp(C.byref(r), None), lambda: lib.hiertcn_preference_loss(C.byref(r), C.byref(q), None),
                  lambda: lib.hiertcn_policy_loss(C.byref(r), C.byref(o), None)):
         assert call() == -1 and b"at most 2^31 - 4097" in lib.hiertcn_ops_last_error()
+
+
+@pytest.fixture
+def steps(monkeypatch):
+    """AdamW on host tensors: what each call of the library is given, as (function, the descriptors' fields) instead of the call."""
+    seen = []
+
+    def call(fn, device, desc, n, *rest):
+        seen.append((fn, [{f: getattr(d, f) for f, _ in _ops.AdamwTensor._fields_} for d in desc]))
+    monkeypatch.setattr(_ops, "on_gpu", lambda t, name: t.device)
+    monkeypatch.setattr(_ops, "call", call)
+    return seen
+
+
+def named(opt, grads):
+    lists = dict(param=opt.params, grad=grads, copy=opt.copies, m=opt.m, v=opt.v, m_scale=opt.m_scale, v_scale=opt.v_scale)
+    return {f: [None if t is None else t.data_ptr() for t in ts] for f, ts in lists.items() if ts is not None}
+
+
+def given(seen, lists):
+    return {f: [d[f] for d in seen[-1][1]] for f in lists}
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_follows_tensors_to_other_memory(lib, steps, bits):
+    from hiertcn_amd.adamw import AdamW
+    k = (700, 40)
+    t = lambda dt, block=1: [torch.zeros(-(-n // block), dtype=dt) for n in k]  # noqa: E731
+    params, grads, copies = t(torch.float32), t(torch.float32), [torch.zeros(700, dtype=torch.bfloat16), None]
+    state = (t(torch.float32), t(torch.float32)) if bits == 32 else (t(torch.int8), t(torch.uint8), t(torch.float32, 256), t(torch.float32, 256))
+    opt = AdamW(params, grads, copies=copies, state_bits=bits, state=state)
+    opt.step()
+    assert given(steps, named(opt, grads)) == named(opt, grads)
+    keep = []
+    for change in (params, grads, copies[:1], *state):
+        for x in change:
+            before, keep = x.data_ptr(), [*keep, x.data]
+            x.data = torch.ones_like(x)
+            assert x.data_ptr() != before
+            opt.step()
+            assert given(steps, named(opt, grads)) == named(opt, grads)
+    params[0].data = torch.zeros(900).resize_(700).clone()
+    params[1].set_(torch.zeros(60)[7:47])
+    opt.moments()
+    opt.step()
+    assert given(steps, named(opt, grads)) == named(opt, grads)
+    taken, n = opt.t, len(steps)
+    bad = [(torch.zeros(701), "701 elements"), (torch.zeros(700, dtype=torch.float64), "dtype"), (torch.zeros(1400)[::2], "contiguous")]
+    for data, word in bad + [(opt.m[0].data, "overlap")] * (bits == 32):
+        good, params[0].data = params[0].data, data
+        for _ in range(2):
+            with pytest.raises(HierTCNError, match=word):
+                opt.step()
+        params[0].data = good
+    good, grads[1].data = grads[1].data, torch.zeros(41)
+    for _ in range(2):                       # refused every time, not taken half-way
+        with pytest.raises(HierTCNError, match=r"grads\[1\]"):
+            opt.step()
+    assert opt.t == taken and len(steps) == n
+    grads[1].data = good
+    opt.step()
+    assert opt.t == taken + 1 and given(steps, named(opt, grads)) == named(opt, grads)
+
+
+def test_adamw_holds_the_memory_that_it_names(lib, steps):
+    """Until it has looked again, what the descriptors name is not handed out to anybody else."""
+    from hiertcn_amd.adamw import AdamW
+    p, g = torch.zeros(1 << 16), torch.zeros(1 << 16)
+    opt = AdamW([p], [g])
+    at = p.data_ptr()
+    p.data = torch.zeros(1 << 16)
+    held = [torch.zeros(1 << 16) for _ in range(20)]
+    assert all(x.data_ptr() != at for x in (*held, p)) and any(x.data_ptr() == at for x in opt._held)
+    opt.step()
+    assert all(x.data_ptr() != at for x in opt._held) and steps[-1][1][0]["param"] == p.data_ptr()
