@@ -2,6 +2,7 @@
 (Engine.adam_step, model.py:139), which has neither.  Kernel: csrc/adamw.hip; exact formulas: include/hiertcn_ops.h."""
 from __future__ import annotations
 
+import bisect
 import ctypes as C
 from typing import List, Optional, Sequence, Union
 
@@ -15,12 +16,25 @@ BLOCK = 256      # elements that share a scale of the 8-bit states
 _address = torch.Tensor.data_ptr
 
 
+def _spans(lists):
+    return sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name, i) for name, ts in lists for i, t in enumerate(ts or ()) if t is not None and t.numel())
+
+
 def _apart(lists):
-    """Refuses two tensors of the lists that share memory: every one is written by waves of its own."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name, i) for name, ts in lists for i, t in enumerate(ts or ()) if t is not None and t.numel())
+    """Refuses two tensors of the lists that share memory: every one is written by waves of its own.  -> where they lie, in order"""
+    spans = _spans(lists)
     for (_, end, a, i), (start, _, b, j) in zip(spans, spans[1:]):
         if start < end:
             raise HierTCNError(f"{a}[{i}] and {b}[{j}] overlap")
+    return spans
+
+
+def _clear_of(spans, starts, lists):
+    """Refuses a tensor of the lists that shares memory with one of `spans` (of _apart; starts: their first addresses)."""
+    for start, end, name, i in _spans(lists):
+        k = bisect.bisect_left(starts, end) - 1
+        if k >= 0 and spans[k][1] > start:
+            raise HierTCNError(f"{name}[{i}] and {spans[k][2]}[{spans[k][3]}] overlap")
 
 
 class AdamW:
@@ -98,7 +112,7 @@ class AdamW:
             if c is not None and (not isinstance(c, torch.Tensor) or c.dtype not in (torch.bfloat16, torch.float16)):
                 raise HierTCNError(f"copies[{i}]: a bfloat16 or float16 tensor")
             rows.append((p.data_ptr(), None, 0) if c is None else (p.data_ptr(), need(c, f"copies[{i}]", c.dtype, self.device, p.shape).data_ptr(), _ops.DTYPE[c.dtype]))
-        _apart((("params", self.params), ("copies", self.copies), ("m", m), ("v", v), ("m_scale", m_scale), ("v_scale", v_scale)))
+        spans = _apart((("params", self.params), ("copies", self.copies), ("m", m), ("v", v), ("m_scale", m_scale), ("v_scale", v_scale)))
         for (name, _, _, _), ptrs in zip(names, found):
             for d, ptr in zip(self._desc, ptrs):
                 setattr(d, name, ptr)
@@ -106,6 +120,8 @@ class AdamW:
             d.param, d.copy, d.copy_dtype = row
         self.m, self.v, self.m_scale, self.v_scale = m, v, m_scale, v_scale
         self._shapes = [p.shape for p in self.params]
+        self._written, self._starts = spans, [s[0] for s in spans]        # what a step writes
+        self._clear = {}                                                  # addresses of gradients / outputs that were last found clear of it
         self._watch()
 
     def _watch(self):
@@ -175,6 +191,9 @@ class AdamW:
             if g is not None and (not isinstance(g, torch.Tensor) or g.dtype not in _ops.DTYPE):
                 raise HierTCNError(f"grads[{i}]: a float32, bfloat16 or float16 tensor")
             found.append((None, 0) if g is None else (need(g, f"grads[{i}]", g.dtype, self.device, shape).data_ptr(), _ops.DTYPE[g.dtype]))
+        if self._clear.get("grads") != found:         # (sizes are the parameters')
+            _clear_of(self._written, self._starts, (("grads", grads),))
+            self._clear["grads"] = found
         for d, (ptr, dtype) in zip(self._desc, found):
             d.grad, d.grad_dtype = ptr, dtype
 
@@ -217,6 +236,10 @@ class AdamW:
             out = tuple([torch.empty(p.numel(), dtype=torch.float32, device=self.device) for p in self.params] for _ in range(2))
         if len(out[0]) != n or len(out[1]) != n:
             raise HierTCNError(f"{n} parameters, outputs for {len(out[0])} and {len(out[1])}")
-        ptrs = [(C.c_void_p * n)(*[None if o is None else need(o, "out", torch.float32, self.device, k).data_ptr() for o, k in zip(lst, self._flat)]) for lst in out]
-        _ops.call(_ops.lib().hiertcn_adamw_moments, self.device, self._desc, n, *ptrs)
+        found = [[None if o is None else need(o, "out", torch.float32, self.device, k).data_ptr() for o, k in zip(lst, self._flat)] for lst in out]
+        if self._clear.get("out") != found:
+            _apart((("m out", out[0]), ("v out", out[1])))
+            _clear_of(self._written, self._starts, (("m out", out[0]), ("v out", out[1])))
+            self._clear["out"] = found
+        _ops.call(_ops.lib().hiertcn_adamw_moments, self.device, self._desc, n, *((C.c_void_p * n)(*ptrs) for ptrs in found))
         return out

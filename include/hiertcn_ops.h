@@ -152,7 +152,8 @@ typedef struct {
 } hiertcn_adamw_t;
 /* tensors: HOST array, read before the call returns.  The buffers of different tensors do not overlap (those of one are checked). */
 int hiertcn_adamw_step(const hiertcn_adamw_tensor_t* tensors, int64_t n, const hiertcn_adamw_t* a, void* stream);
-/* the values of 8-bit states: m_out[i], v_out[i] (HOST arrays of device float pointers, an entry may be NULL) */
+/* the values of 8-bit states: m_out[i], v_out[i] (HOST arrays of device float pointers, an entry may be NULL), which overlap neither one another nor anything of
+ * the tensors (those of one tensor are checked against its states) */
 int hiertcn_adamw_moments(const hiertcn_adamw_tensor_t* tensors, int64_t n, float* const* m_out, float* const* v_out, void* stream);
 /* after another optimizer has changed a training handle's masters (hiertcn_train_arena 0): the 16-bit device copies, as hiertcn_adam_step refreshes them.
  * (A call on a handle: its message is in hiertcn_last_error().) */

@@ -432,3 +432,48 @@ def test_adamw_holds_the_memory_that_it_names(lib, steps):
     assert all(x.data_ptr() != at for x in (*held, p)) and any(x.data_ptr() == at for x in opt._held)
     opt.step()
     assert all(x.data_ptr() != at for x in opt._held) and steps[-1][1][0]["param"] == p.data_ptr()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_refuses_gradients_inside_what_it_writes(lib, steps, bits):
+    """A gradient that shares memory with ANOTHER tensor's parameter, copy or state would be read while that is written; gradients may share among themselves."""
+    from hiertcn_amd.adamw import AdamW
+    buf = torch.zeros(1000)
+    params, copies = [buf[:300], buf[300:600]], [torch.zeros(300, dtype=torch.bfloat16) for _ in range(2)]
+    opt = AdamW(params, copies=copies, state_bits=bits)
+    same = torch.zeros(300)
+    opt.step([same, same])
+    n, t = len(steps), opt.t
+    bad = [([buf[299:599], None], "params"), ([None, buf[:300]], "params"), ([copies[1], None], "copies")]
+    if bits == 32:
+        bad.append(([None, opt.v[0]], "v"))
+    for grads, name in bad:
+        for call in (lambda: opt.step(grads), lambda: AdamW(params, grads, copies=copies) if name != "v" else opt.step(grads)):
+            with pytest.raises(HierTCNError, match=rf"grads\[.\] and {name}\[.\] overlap"):
+                call()
+    assert len(steps) == n and opt.t == t
+    opt.step([buf[700:], None])
+    opt.step([same, same])
+    assert opt.t == t + 2
+    params[1].data = same                     # the parameter comes to where a gradient that was clear lies
+    with pytest.raises(HierTCNError, match=r"grads\[.\] and params\[1\] overlap"):
+        opt.step([same, None])
+
+
+def test_adamw_moments_refuses_outputs_inside_one_another_or_what_it_writes(lib, steps):
+    from hiertcn_amd.adamw import AdamW
+    params = [torch.zeros(300), torch.zeros(256)]
+    opt = AdamW(params, state_bits=8)
+    z = lambda: [torch.zeros(300), torch.zeros(256)]  # noqa: E731
+    m, v = z(), z()
+    buf = torch.zeros(512)
+    for out, word in (((m, [m[0], v[1]]), "overlap"), (([m[0], buf[:256]], [v[0], buf[255:511]]), "overlap"), (([params[0], m[1]], v), "params"),
+                      (([None, params[1]], [None, None]), "params"), (([m[0], params[0][:256]], v), "params")):
+        n = len(steps)
+        with pytest.raises(HierTCNError, match=word):
+            opt.moments(out=out)
+        assert len(steps) == n
+    for _ in range(2):
+        opt.moments(out=(m, v))
+        opt.moments(out=([None, buf[:256]], [v[0], buf[256:]]))
+    assert len(steps) == 4
