@@ -223,6 +223,9 @@ class AdamW:
     def moments(self, out=None):
         """-> (m, v): lists of flat fp32 tensors -- the states themselves (32 bits), or the values that the codes stand for, written to `out` = (list, list)
         where that is given (entries of None are skipped)."""
+        n = len(self.params)
+        if out is not None and (len(out[0]) != n or len(out[1]) != n):
+            raise HierTCNError(f"{n} parameters, outputs for {len(out[0])} and {len(out[1])}")
         if self.state_bits == 32:
             if out is not None:
                 for dst, src in zip((*out[0], *out[1]), (*self.m, *self.v)):
@@ -231,11 +234,8 @@ class AdamW:
                 return out
             return self.m, self.v
         self._follow(states_only=True)
-        n = len(self.params)
         if out is None:
             out = tuple([torch.empty(p.numel(), dtype=torch.float32, device=self.device) for p in self.params] for _ in range(2))
-        if len(out[0]) != n or len(out[1]) != n:
-            raise HierTCNError(f"{n} parameters, outputs for {len(out[0])} and {len(out[1])}")
         found = [[None if o is None else need(o, "out", torch.float32, self.device, k).data_ptr() for o, k in zip(lst, self._flat)] for lst in out]
         if self._clear.get("out") != found:
             _apart((("m out", out[0]), ("v out", out[1])))

@@ -477,3 +477,21 @@ def test_adamw_moments_refuses_outputs_inside_one_another_or_what_it_writes(lib,
         opt.moments(out=(m, v))
         opt.moments(out=([None, buf[:256]], [v[0], buf[256:]]))
     assert len(steps) == 4
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_moments_takes_one_output_a_tensor(lib, steps, bits):
+    """Lists of another length are refused in both forms of the states (entries of None are skipped)."""
+    from hiertcn_amd.adamw import AdamW
+    params = [torch.zeros(5), torch.zeros(5)]
+    opt = AdamW(params, state_bits=bits)
+    z = lambda: torch.zeros(5)  # noqa: E731
+    for out in (([z()], [z(), z()]), ([z(), z(), z()], [z()])):
+        with pytest.raises(HierTCNError):
+            opt.moments(out=out)
+    if bits == 32:
+        opt.m[1].fill_(2.0)
+        opt.v[0].fill_(3.0)
+        out = ([None, z()], [z(), None])
+        opt.moments(out=out)
+        assert (out[0][1] == 2).all() and (out[1][0] == 3).all()
