@@ -23,6 +23,7 @@ namespace {
 constexpr int NT = 256, BLOCK = 256;     // threads of a workgroup; elements of a block (one wave, four to a lane)
 constexpr int PER_WG = NT / 64;          // blocks of a workgroup
 constexpr int MAX_TENSORS = 40;          // of a launch: 40 descriptors fit the 4 KB of kernel arguments
+constexpr uint32_t PIECE = 1u << 23;     // workgroups of a tensor in one launch, at most: a longer tensor goes in pieces
 
 struct Batch {
   hiertcn_adamw_tensor_t t[MAX_TENSORS];
@@ -33,6 +34,7 @@ struct Batch {
   const float* gscale_dev;
   uint32_t key;                          // of the random bits, without the tensor's share
   uint64_t wide;                         // bit i: tensor i's addresses allow four elements at a time
+  uint32_t zero[MAX_TENSORS];            // where the tensor's own first workgroup would lie: first, less those of the pieces before (modulo 2^32)
 };
 static_assert(sizeof(Batch) <= 4096, "kernel arguments");
 
@@ -248,7 +250,7 @@ __device__ __forceinline__ void update(const Batch& b, const hiertcn_adamw_tenso
 // the wave's first block of its tensor, of EACH.  false: behind its end
 template <int EACH, typename B>
 __device__ __forceinline__ bool block_here(const B& b, int i, int64_t& block) {
-  block = ((int64_t)(blockIdx.x - b.first[i]) * PER_WG + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * EACH;
+  block = ((int64_t)(blockIdx.x - b.zero[i]) * PER_WG + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * EACH;
   return block * BLOCK < b.t[i].numel;
 }
 template <bool Q8>
@@ -266,6 +268,7 @@ struct DecodeBatch {
   uint32_t first[MAX_TENSORS + 1];
   int n;
   uint64_t wide;
+  uint32_t zero[MAX_TENSORS];
 };
 static_assert(sizeof(DecodeBatch) <= 4096, "kernel arguments");
 // a wave decodes WAVE_BLOCKS blocks of a tensor, all loads first
@@ -328,6 +331,39 @@ int check_tensor(const hiertcn_adamw_tensor_t& t, int64_t i, bool q8, bool need_
   }
   return HIERTCN_OK;
 }
+// The launches of a call, one after the other: which pieces of which tensors go into the next one, `each` blocks to a wave.  All that a call can refuse is
+// refused before the first of them.
+struct Walk {
+  const hiertcn_adamw_tensor_t* t;
+  int64_t n, i, piece;
+  int each;
+  int64_t tensor[MAX_TENSORS];           // the launch at hand
+  uint32_t first[MAX_TENSORS + 1];
+  uint8_t which[MAX_TENSORS];
+  int count;
+  Walk(const hiertcn_adamw_tensor_t* t, int64_t n, int each) : t(t), n(n), i(0), piece(0), each(each), count(0) {}
+  // works(i): whether tensor i takes part.  -> its number of workgroups, 0 behind the last
+  template <typename F>
+  uint32_t next(F works) {
+    int64_t wgs = 0;
+    for (count = 0; i < n && count < MAX_TENSORS;) {
+      if (t[i].numel == 0 || !works(i)) {
+        i++;
+        continue;
+      }
+      const int64_t span = (int64_t)BLOCK * PER_WG * each, all = (t[i].numel + span - 1) / span, left = all - piece * PIECE, w = left < PIECE ? left : PIECE;
+      if (wgs + w > ops_most_groups(NT)) break;
+      tensor[count] = i;
+      first[count] = (uint32_t)wgs;
+      which[count++] = (uint8_t)piece;
+      wgs += w;
+      if (w < left) piece++;
+      else i++, piece = 0;
+    }
+    first[count] = (uint32_t)wgs;
+    return (uint32_t)wgs;
+  }
+};
 bool wide_of(const hiertcn_adamw_tensor_t& t, bool q8) {
   const size_t ss = q8 ? 4 : 16;
   return (uintptr_t)t.param % 16 == 0 && (uintptr_t)t.m % ss == 0 && (uintptr_t)t.v % ss == 0 && (uintptr_t)t.copy % 8 == 0 &&
@@ -364,27 +400,21 @@ int hiertcn_adamw_step(const hiertcn_adamw_tensor_t* tensors, int64_t n, const h
   b.gscale = (float)a->grad_scale;
   b.gscale_dev = a->grad_scale_dev;
   b.key = (uint32_t)((uint64_t)a->seed * 0x9E3779B1u + (uint64_t)a->t * 0x6A09E667u);
-  for (int64_t i = 0; i < n;) {
-    b.n = 0;
+  Walk walk(tensors, n, 1);
+  while (const uint32_t wgs = walk.next([&](int64_t i) { return tensors[i].grad != nullptr; })) {
+    b.n = walk.count;
     b.wide = 0;
-    uint64_t wgs = 0;
-    for (; i < n && b.n < MAX_TENSORS; i++) {
-      const hiertcn_adamw_tensor_t& t = tensors[i];
-      if (t.numel == 0 || !t.grad) continue;
-      const uint64_t blocks = (uint64_t)(t.numel + BLOCK - 1) / BLOCK, w = (blocks + PER_WG - 1) / PER_WG;
-      if (w > 0x7fffffffull) return ops_fail(HIERTCN_ERR_INVALID, "tensor %lld: too large for one launch", (long long)i);
-      if (wgs + w > 0x7fffffffull) break;
-      b.t[b.n] = t;
-      b.decay[b.n] = (float)(1.0 - a->lr * t.weight_decay);
-      b.first[b.n] = (uint32_t)wgs;
-      if (wide_of(t, q8)) b.wide |= 1ull << b.n;
-      b.n++;
-      wgs += w;
+    for (int k = 0; k < b.n; k++) {
+      const hiertcn_adamw_tensor_t& t = tensors[walk.tensor[k]];
+      b.t[k] = t;
+      b.decay[k] = (float)(1.0 - a->lr * t.weight_decay);
+      b.first[k] = walk.first[k];
+      b.zero[k] = walk.first[k] - walk.which[k] * PIECE;
+      if (wide_of(t, q8)) b.wide |= 1ull << k;
     }
-    if (!b.n) continue;
-    b.first[b.n] = (uint32_t)wgs;
-    if (q8) hipLaunchKernelGGL((k_adamw<true>), dim3((unsigned)wgs), dim3(NT), 0, st, b);
-    else hipLaunchKernelGGL((k_adamw<false>), dim3((unsigned)wgs), dim3(NT), 0, st, b);
+    b.first[b.n] = wgs;
+    if (q8) hipLaunchKernelGGL((k_adamw<true>), dim3(wgs), dim3(NT), 0, st, b);
+    else hipLaunchKernelGGL((k_adamw<false>), dim3(wgs), dim3(NT), 0, st, b);
     OPS_TRY(hipGetLastError());
   }
   return HIERTCN_OK;
@@ -403,27 +433,44 @@ int hiertcn_adamw_moments(const hiertcn_adamw_tensor_t* tensors, int64_t n, floa
     if (ops_overlap(mo, vo)) return ops_fail(HIERTCN_ERR_INVALID, "tensor %lld: the outputs overlap", (long long)i);
   }
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  for (int64_t i = 0; i < n;) {
+  Walk walk(tensors, n, WAVE_BLOCKS);
+  while (const uint32_t wgs = walk.next([&](int64_t i) { return m_out[i] || v_out[i]; })) {
     DecodeBatch b{};
-    uint64_t wgs = 0;
-    for (; i < n && b.n < MAX_TENSORS; i++) {
+    b.n = walk.count;
+    for (int k = 0; k < b.n; k++) {
+      const int64_t i = walk.tensor[k];
       const hiertcn_adamw_tensor_t& t = tensors[i];
-      if (t.numel == 0 || (!m_out[i] && !v_out[i])) continue;
-      const uint64_t blocks = (uint64_t)(t.numel + BLOCK - 1) / BLOCK, w = (blocks + PER_WG * WAVE_BLOCKS - 1) / (PER_WG * WAVE_BLOCKS);
-      if (w > 0x7fffffffull) return ops_fail(HIERTCN_ERR_INVALID, "tensor %lld: too large for one launch", (long long)i);
-      if (wgs + w > 0x7fffffffull) break;
-      b.t[b.n] = {t.numel, t.m, t.v, t.m_scale, t.v_scale, m_out[i], v_out[i]};
-      b.first[b.n] = (uint32_t)wgs;
-      if ((uintptr_t)t.m % 4 == 0 && (uintptr_t)t.v % 4 == 0 && (uintptr_t)m_out[i] % 16 == 0 && (uintptr_t)v_out[i] % 16 == 0) b.wide |= 1ull << b.n;
-      b.n++;
-      wgs += w;
+      b.t[k] = {t.numel, t.m, t.v, t.m_scale, t.v_scale, m_out[i], v_out[i]};
+      b.first[k] = walk.first[k];
+      b.zero[k] = walk.first[k] - walk.which[k] * PIECE;
+      if ((uintptr_t)t.m % 4 == 0 && (uintptr_t)t.v % 4 == 0 && (uintptr_t)m_out[i] % 16 == 0 && (uintptr_t)v_out[i] % 16 == 0) b.wide |= 1ull << k;
     }
-    if (!b.n) continue;
-    b.first[b.n] = (uint32_t)wgs;
-    hipLaunchKernelGGL(k_moments, dim3((unsigned)wgs), dim3(NT), 0, st, b);
+    b.first[b.n] = wgs;
+    hipLaunchKernelGGL(k_moments, dim3(wgs), dim3(NT), 0, st, b);
     OPS_TRY(hipGetLastError());
   }
   return HIERTCN_OK;
 }
+
+#ifdef HIERTCN_TEST_HOOKS       // (the launches of a call on tensors of these sizes, for a test on the host: rows of launch, tensor, piece, first workgroup, the launch's workgroups)
+int64_t hiertcn_test_adamw_walk(const int64_t* numel, int64_t n, int each, int64_t* out, int64_t room) {
+  hiertcn_adamw_tensor_t t[256] = {};
+  if (n > 256) return -1;
+  for (int64_t i = 0; i < n; i++) t[i].numel = numel[i];
+  Walk walk(t, n, each);
+  int64_t rows = 0, launch = 0;
+  for (; const uint32_t wgs = walk.next([](int64_t) { return true; }); launch++)
+    for (int k = 0; k < walk.count; k++, rows++) {
+      if (rows == room) return -1;
+      const int64_t row[5] = {launch, walk.tensor[k], walk.which[k], walk.first[k], wgs};
+      for (int x = 0; x < 5; x++) out[5 * rows + x] = row[x];
+    }
+  return rows;
+}
+int hiertcn_test_adamw_sizes(int64_t out[4]) {
+  out[0] = PIECE, out[1] = BLOCK * PER_WG, out[2] = MAX_TENSORS, out[3] = NT;
+  return WAVE_BLOCKS;
+}
+#endif
 
 }  // extern "C"

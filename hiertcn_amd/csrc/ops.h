@@ -13,6 +13,9 @@ int ops_fail(int code, const char* fmt, ...);   // sets this thread's message, r
     if (e_ != hipSuccess) return ops_fail(HIERTCN_ERR_HIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__, __LINE__);       \
   } while (0)
 
+// workgroups of a launch, at most: HIP counts its threads in 32 bits
+constexpr int64_t ops_most_groups(int threads) { return 0xffffffffll / threads; }
+
 static inline int ops_size(int dtype) { return dtype == HIERTCN_FP32 ? 4 : 2; }
 static inline bool ops_dtype_ok(int dtype) { return dtype >= HIERTCN_FP32 && dtype <= HIERTCN_FP16; }
 

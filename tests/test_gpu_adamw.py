@@ -274,3 +274,36 @@ def test_parameters_that_moved(bits):
     b.step()
     assert all(torch.equal(x, y) for x, y in zip(params + copies + list(a.m), twin + tcopies + list(b.m)))
     assert all(torch.equal(o, k) for o, k in zip(old, kept)) and not torch.equal(params[0], kept[0])
+
+
+def test_a_tensor_of_more_blocks_than_a_launch_takes():
+    """2^34 + 700 elements: 2^24 + 1 workgroups, more than a launch may have.  First, middle and last blocks of the step and of the decoded moments as the formula says."""
+    from hiertcn_amd.adamw import AdamW
+    if torch.cuda.mem_get_info()[0] < 170 << 30:
+        pytest.skip("170 GiB of device memory")
+    n, lr = 2 ** 34 + 700, 1e-2
+    p = torch.full((n,), 0.5, device="cuda")
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    edge = 2 ** 33                                         # where the second piece of the step begins
+    spots = [(0, 512), (edge - 512, 1024), (2 ** 34 - 256, 956)]
+    rng = np.random.default_rng(6)
+    grads = []
+    for at, k in spots:
+        grads.append(torch.tensor(rng.standard_normal(k), dtype=torch.float32).to(torch.bfloat16))
+        g[at:at + k] = grads[-1].cuda()
+    opt = AdamW([p], [g], lr=lr, betas=(B1, B2), eps=E, state_bits=8, seed=9)
+    opt.step()
+    for (at, k), grad in zip(spots, grads):
+        blocks = -(-k // 256)
+        zero = np.zeros(blocks, np.float32)
+        whole = SO.mix
+        try:
+            SO.mix = lambda numel, tensor, t, seed, at=at: _bits(at + np.arange(numel, dtype=np.uint64), t, seed)
+            q, qm, qv, sm, sv = SO.adamw8(np.full(k, 0.5, np.float32), grad.float().numpy(), np.zeros(k, np.int8), np.zeros(k, np.uint8), zero, zero, 1, lr, B1, B2, E, 0.0, 9, 0)
+        finally:
+            SO.mix = whole
+        b0 = at // 256
+        for got, want in ((opt.m[0][at:at + k], qm), (opt.v[0][at:at + k], qv), (opt.m_scale[0][b0:b0 + blocks], sm), (opt.v_scale[0][b0:b0 + blocks], sv)):
+            assert np.array_equal(got.cpu().numpy(), want), at
+        assert (np.abs(p[at:at + k].cpu().numpy() - q) <= 4 * EPS * (np.abs(q) + 1e-2)).all()
+    assert (p[512:edge - 512] == 0.5).all() and (p[edge + 512:2 ** 34 - 256] == 0.5).all()

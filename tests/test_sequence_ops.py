@@ -495,3 +495,38 @@ def test_adamw_moments_takes_one_output_a_tensor(lib, steps, bits):
         out = ([None, z()], [z(), None])
         opt.moments(out=out)
         assert (out[0][1] == 2).all() and (out[1][0] == 3).all()
+
+
+def test_adamw_launches_cover_every_block_within_the_limits():
+    """The launches of a call (the test-hook build names them): every workgroup of every tensor once, at most 40 tensors and fewer than 2^32 threads a launch -- HIP's
+    limit on the threads of a dimension -- for one tensor of 2^40 elements as for many."""
+    import itertools
+    from hiertcn_amd.build import LIB_TESTHOOKS
+    so = C.CDLL(LIB_TESTHOOKS)
+    so.hiertcn_test_adamw_walk.restype = C.c_int64
+    so.hiertcn_test_adamw_walk.argtypes = [C.POINTER(C.c_int64), C.c_int64, C.c_int, C.POINTER(C.c_int64), C.c_int64]
+    sizes = (C.c_int64 * 4)()
+    each_moments = so.hiertcn_test_adamw_sizes(sizes)
+    piece, span, most, threads = sizes
+    G = 1 << 30
+    cases = [[1], [0, 5, 0, 257], list(range(1, 150)), [1 << 40], [16 * G - 1], [16 * G], [16 * G + 1024, 3], [17 * G] * 5, [8 * G] * 3 + [1], [3 * G] * 41, [(1 << 40) - 1, 70, 1 << 40]]
+    for numel, each in itertools.product(cases, (1, each_moments)):
+        out = (C.c_int64 * 50000)()
+        rows = so.hiertcn_test_adamw_walk((C.c_int64 * len(numel))(*numel), len(numel), each, out, 10000)
+        assert rows > 0
+        rows = np.array(out[:5 * rows]).reshape(-1, 5)
+        assert (rows[:, 2] < 256).all() and (rows[:, 4] * threads < 2 ** 32).all()
+        done = {i: [] for i in range(len(numel))}
+        for launch in range(rows[-1, 0] + 1):
+            mine = rows[rows[:, 0] == launch]
+            assert 0 < len(mine) <= most and (mine[:, 4] == mine[0, 4]).all() and mine[0, 3] == 0
+            ends = np.append(mine[1:, 3], mine[0, 4])
+            assert (ends > mine[:, 3]).all()
+            for (_, tensor, which, first, _), end in zip(mine, ends):
+                done[tensor].append((which * piece, which * piece + end - first))
+        for i, k in enumerate(numel):
+            want, at = -(-k // (span * each)), 0
+            for start, end in done[i]:              # in order, side by side
+                assert start == at
+                at = end
+            assert at == want, (numel, i)
