@@ -493,6 +493,10 @@ size_t workspace_of(int64_t n, int64_t T, int64_t V, RowsP* p) {
   const size_t groups = (R + NT / lanes - 1) / (NT / lanes);
   const size_t sizes[6] = {align_up(R * most * 8), align_up(R * 8), align_up(R * 4), align_up(groups * 24), align_up((size_t)n * 4), align_up((size_t)counters_of(n, T) * 16)};
   if (p) {
+    p->lanes = lanes;
+    p->groups = (int64_t)groups;
+  }
+  if (p && p->a.workspace) {
     char* w = static_cast<char*>(p->a.workspace);
     p->part = reinterpret_cast<float2*>(w);
     p->stat = reinterpret_cast<float2*>(w += sizes[0]);
@@ -500,8 +504,6 @@ size_t workspace_of(int64_t n, int64_t T, int64_t V, RowsP* p) {
     p->term = reinterpret_cast<double*>(w += sizes[2]);
     p->count = reinterpret_cast<int32_t*>(w += sizes[3]);
     p->total = reinterpret_cast<int64_t*>(w += sizes[4]);
-    p->lanes = lanes;
-    p->groups = (int64_t)groups;
   }
   return sizes[0] + sizes[1] + sizes[2] + sizes[3] + sizes[4] + sizes[5];
 }
@@ -520,6 +522,16 @@ int prepare(const hiertcn_rows_t* in, bool grad, RowsP& p, int& vec) {
   if (p.R == 1) a.ld = a.V, a.dld = a.dlogits ? a.V : 0;
   if (a.ld < a.V || a.ld > (1ll << 40) || (a.dlogits && (a.dld < a.V || a.dld > (1ll << 40)))) return ops_fail(HIERTCN_ERR_INVALID, "a row stride is smaller than V");
   const int es = ops_size(a.dtype);
+  // 16 bytes at a time wherever the two passes' rows are 16-byte aligned alike; else one element
+  vec = 16 / es;
+  if (a.dlogits && (((uintptr_t)a.logits - (uintptr_t)a.dlogits) % 16 || (a.ld - a.dld) % vec)) vec = 1;
+  p.read = read_of(p.R, a.V, vec);
+  p.write = cut_of(p.R, a.V, vec, PART);
+  p.counters = 0;
+  workspace_of(a.n, a.T, a.V, &p);      // (addresses into a workspace that is checked below)
+  const int64_t most = ops_most_groups(NT);
+  if (workgroups(p.read, p.R) + counters_of(a.n, a.T) > most || workgroups(p.write, p.R) + 1 > most || p.groups > most)
+    return ops_fail(HIERTCN_ERR_INVALID, "%lld rows of %lld are too many for one launch: at most 2^24 - 1 workgroups of a part of a row, or of four short rows", (long long)p.R, (long long)a.V);
   if ((uintptr_t)a.logits % es || (uintptr_t)a.dlogits % es || (uintptr_t)a.ids % 4 || (uintptr_t)a.logp % 4)
     return ops_fail(HIERTCN_ERR_INVALID, "a pointer is not a multiple of its element");
   if (!(a.grad_scale - a.grad_scale == 0.f)) return ops_fail(HIERTCN_ERR_INVALID, "grad_scale is not finite");
@@ -532,14 +544,6 @@ int prepare(const hiertcn_rows_t* in, bool grad, RowsP& p, int& vec) {
   for (const OpsView* o : {&lp, &ws})
     if (ops_overlap(*o, z) || ops_overlap(*o, ids) || ops_overlap(*o, d)) return ops_fail(HIERTCN_ERR_INVALID, "logp or the workspace overlaps another operand");
   if (ops_overlap(lp, ws) || ops_overlap(ids, d)) return ops_fail(HIERTCN_ERR_INVALID, "logp or the workspace overlaps another operand");
-  // 16 bytes at a time wherever the two passes' rows are 16-byte aligned alike; else one element
-  vec = 16 / es;
-  if (a.dlogits && (((uintptr_t)a.logits - (uintptr_t)a.dlogits) % 16 || (a.ld - a.dld) % vec)) vec = 1;
-  p.read = read_of(p.R, a.V, vec);
-  p.write = cut_of(p.R, a.V, vec, PART);
-  p.counters = 0;
-  workspace_of(a.n, a.T, a.V, &p);
-  if (workgroups(p.read, p.R) + a.n > 0x7fffffffll || workgroups(p.write, p.R) + a.n > 0x7fffffffll) return ops_fail(HIERTCN_ERR_INVALID, "n * T * V is too large for one launch");
   return HIERTCN_OK;
 }
 
@@ -605,6 +609,7 @@ int hiertcn_preference_loss(const hiertcn_rows_t* r, const hiertcn_preference_t*
   if (!q) return ops_fail(HIERTCN_ERR_INVALID, "null argument");
   if (int rc = prepare(r, true, p, vec)) return rc;
   const int64_t n = p.a.n, P = n / 2;
+  if (P > ops_most_groups(PAIR_NT)) return ops_fail(HIERTCN_ERR_INVALID, "%lld pairs: at most 2^22 - 1", (long long)P);
   if (n % 2) return ops_fail(HIERTCN_ERR_INVALID, "%lld sequences: pairs are wanted", (long long)n);
   if (q->kind < 0 || q->kind > 2) return ops_fail(HIERTCN_ERR_INVALID, "kind %d: 0 sigmoid, 1 hinge, 2 squared", q->kind);
   if (!(q->beta > 0.f) || q->beta > 3e38f) return ops_fail(HIERTCN_ERR_INVALID, "beta has to be positive and finite");

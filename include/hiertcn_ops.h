@@ -70,7 +70,8 @@ int hiertcn_glr_backward(const hiertcn_glr_t* a, void* stream);
 /* ---- losses on the log-probabilities of answers, with their gradients ----------------------------------------------------------------------
  * logits [n * T][V] of n sequences (row stride ld >= V elements), ids [n * T]: the item answered with at every step, 0 = none (padding).  A row whose id
  * lies outside 1 .. V-1 is not read, has log-probability 0 and gradient 0; so is a row of nothing but -inf (no distribution is left).  Column 0 takes part in
- * the soft-max, as in model_tcn.py:41.   logp = z[id] - log sum_j exp z_j.   V is at most 2^31 - 4097.
+ * the soft-max, as in model_tcn.py:41.   logp = z[id] - log sum_j exp z_j.   V is at most 2^31 - 4097,
+ * n T at most 2^24 - 1 rows of more than some hundred or thousand items (of their parts, where a row is cut into up to 64) and about 2^26 shorter ones: what goes into a launch.
  * dlogits (rows of stride dld, the logits' type) may be the logits' own buffer (ptr and stride equal): it is overwritten row by row. */
 typedef struct {
   int64_t n, T, V;
@@ -90,7 +91,7 @@ int hiertcn_sequence_logp(const hiertcn_rows_t* r, void* stream);
  * sequence (divided by its number of answers when `average`; 0 where there is none) and D = (s_i - ref_i) - (s_{P+i} - ref_{P+i}):
  *   kind 0  (1 - smoothing) softplus(-beta D) + smoothing softplus(beta D)
  *   kind 1  max(0, 1 - beta D)
- *   kind 2  (D - 1 / (2 beta))^2
+ *   kind 2  (D - 1 / (2 beta))^2              (P is at most 2^22 - 1)
  * loss [1] = mean of pair_loss; the gradient is that of grad_scale * loss. */
 typedef struct {
   int32_t kind, average;

@@ -530,3 +530,26 @@ def test_adamw_launches_cover_every_block_within_the_limits():
                 assert start == at
                 at = end
             assert at == want, (numel, i)
+
+
+def big_rows(n, T, V, dtype=0):
+    at = lambda k: (1 << 50) + (k << 44)  # noqa: E731
+    return _ops.Rows(n=n, T=T, V=V, dtype=dtype, ld=V, dld=V, grad_scale=1.0, logits=at(0), ids=at(1), logp=at(2), dlogits=at(3), workspace=at(4), workspace_bytes=1 << 43)
+
+
+@pytest.mark.parametrize("n,T,V", [(1 << 13, 1 << 13, 8), (1 << 12, 1 << 12, 9000), (1 << 11, 1 << 10, 600000), (1 << 14, 1 << 12, 20000)])
+def test_losses_refuse_more_rows_than_a_launch_takes(lib, n, T, V):
+    """HIP counts a launch's threads in 32 bits: 2^24 - 1 workgroups of 256.  Refused before the first launch, not by the runtime behind it."""
+    r = big_rows(n, T, V)
+    q = outputs(_ops.Preference(kind=0, beta=0.1), ("ref", "loss", "pair_loss", "margin", "seq_logp"))
+    o = outputs(_ops.Policy(clip_low=0.2, clip_high=0.2), ("old_logp", "advantage", "loss", "kl", "clipped"))
+    for call in (lambda: lib.hiertcn_sequence_logp(C.byref(r), None), lambda: lib.hiertcn_preference_loss(C.byref(r), C.byref(q), None),
+                 lambda: lib.hiertcn_policy_loss(C.byref(r), C.byref(o), None)):
+        assert call() == -1 and b"too many for one launch" in lib.hiertcn_ops_last_error()
+
+
+def test_preference_refuses_more_pairs_than_a_launch_takes(lib):
+    """A workgroup of 1024 threads a pair: 2^22 - 1 of them."""
+    r = big_rows(1 << 23, 1, 4)
+    q = outputs(_ops.Preference(kind=0, beta=0.1), ("ref", "loss", "pair_loss", "margin", "seq_logp"), 1 << 56)
+    assert lib.hiertcn_preference_loss(C.byref(r), C.byref(q), None) == -1 and b"pairs: at most" in lib.hiertcn_ops_last_error()
