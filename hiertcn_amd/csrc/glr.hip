@@ -614,7 +614,8 @@ int glr(const hiertcn_glr_t* in, bool backward, hipStream_t st) {
   p.nseg = (int)nseg;
   p.ncb = (int)q.ncb;
   p.ntile = (int)q.ntile;
-  if (q.ncb * a.B * (q.chain ? q.ntile : 1) > 0x7fffffffll) return ops_fail(HIERTCN_ERR_INVALID, "B * D is too large for one launch");
+  if (q.ncb * a.B * (q.chain ? q.ntile : 1) > ops_most_groups(64 * q.nw))
+    return ops_fail(HIERTCN_ERR_INVALID, "%lld sequences of %lld channels are too many for one launch: B * ceil(D / 64) is at most 2^26 - 1", (long long)a.B, (long long)a.D);
   if (q.chain) {
     const size_t need = workspace_of(a.B, a.T, a.D);      // (the most that any alignment and direction takes)
     if (!a.workspace || a.workspace_bytes < need || (uintptr_t)a.workspace % 16)

@@ -41,7 +41,7 @@ enum hiertcn_dtype { HIERTCN_FP32 = 0, HIERTCN_BF16 = 1, HIERTCN_FP16 = 2 };
  *   backward lambda_t = dout_t + a_{t+1} lambda_{t+1} with a = u [mask != 0] and dstate_out entering behind the last step;
  *            dcand = lambda (1 - u) act'(cand), dgate = lambda (h_prev - c) u (1 - u), dstate_in = a_0 lambda_0; rows behind lengths[b] get 0
  * state_out may be state_in itself.  Other outputs overlap neither each other nor inputs (refused where it can be seen from pointers and strides).
- * B, T, D >= 0 (an empty call copies the state).  workspace: hiertcn_glr_workspace_bytes, 16-byte aligned; 0 where the shape needs none.  (Its workgroups wait for
+ * B, T, D >= 0 (an empty call copies the state), B * ceil(D / 64) at most 2^26 - 1.  workspace: hiertcn_glr_workspace_bytes, 16-byte aligned; 0 where the shape needs none.  (Its workgroups wait for
  * one another through it.  A wait that cannot end -- two calls at once in one workspace -- gives up after some seconds, and what could not be learnt is NaN.) */
 typedef struct {
   int64_t B, T, D;

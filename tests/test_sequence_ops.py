@@ -553,3 +553,16 @@ def test_preference_refuses_more_pairs_than_a_launch_takes(lib):
     r = big_rows(1 << 23, 1, 4)
     q = outputs(_ops.Preference(kind=0, beta=0.1), ("ref", "loss", "pair_loss", "margin", "seq_logp"), 1 << 56)
     assert lib.hiertcn_preference_loss(C.byref(r), C.byref(q), None) == -1 and b"pairs: at most" in lib.hiertcn_ops_last_error()
+
+
+@pytest.mark.parametrize("B,T,D", [(1 << 26, 1, 1), (1 << 27, 3, 64), (1 << 20, 40, 64 * 64)])
+def test_glr_refuses_more_sequences_than_a_launch_takes(lib, B, T, D):
+    """A wave of 64 threads a sequence and 64 channels, where they are many: fewer than 2^26 of them, by HIP's limit on the threads of a launch."""
+    a = _ops.Glr(B=B, T=T, D=D, dtype=0, cand_act=1)
+    for k, f in enumerate(("gate", "cand", "out", "dout", "dgate", "dcand", "state_in", "state_out", "record", "dstate_out", "dstate_in")):
+        setattr(a, f, (1 << 50) + (k << 46) + 4)          # (addresses that allow one channel at a time)
+        if k < 6:
+            setattr(a, f + "_sb", T * D)
+            setattr(a, f + "_st", D)
+    for call in (lib.hiertcn_glr_forward, lib.hiertcn_glr_backward):
+        assert call(C.byref(a), None) == -1 and b"too many for one launch" in lib.hiertcn_ops_last_error(), lib.hiertcn_ops_last_error()
