@@ -301,3 +301,36 @@ def test_an_infinite_state_stays_infinite(T, resets):
     assert torch.isneginf(dx[0, :, 1::2]).all() and torch.isneginf(d0[0, 1::2]).all() and torch.isfinite(dx[:, :, ::2]).all()
     if resets:
         assert torch.isneginf(dx[1, T - 3:, 1::2]).all() and torch.isfinite(dx[1, :T - 3]).all() and torch.isfinite(d0[1]).all()
+
+
+# Two channels a lane from 8192 waves on (B * ceil(D / 128) * ceil(T / 16)): one wave a sequence; several tiles of waves one behind the other; chained workgroups.
+WIDE = [(2100, 64, 128, 60), (310, 450, 130, 14), (2, 33000, 256, 1)]
+
+
+FORMS = [("tanh", True), ("none", False), ("tanh", False), ("none", True)]
+
+
+@pytest.mark.parametrize("shape,act,resets", [(s, *f) for s in WIDE for f in FORMS[:2 if s[1] > 1000 else 4]], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_two_channels_a_lane(shape, dtype, act, resets):
+    """Every `every`-th sequence against 64 bits; the others against the same sequences called by themselves (one channel a lane), to both calls' bounds."""
+    from hiertcn_amd.glr import glr_scan, glr_scan_backward
+    B, T, D, every = shape
+    assert B * -(-D // 128) * -(-T // 16) >= 8192
+    g, x, dh, state, ds, mask, lengths = inputs(B, T, D, dtype, seed=T, resets=resets)
+    h, s, rec = glr_scan(g, x, state, mask=mask, lengths=lengths, cand_act=act, want_record=True)
+    dg, dx, d0 = glr_scan_backward(g, x, dh, rec, mask=mask, lengths=lengths, cand_act=act, dstate_out=ds)
+    pick = torch.arange(0, B, every, device="cuda")
+    of = lambda v: None if v is None else v[pick]  # noqa: E731
+    ref = reference(of(g), of(x), of(state), of(mask), of(lengths), act, of(dh), of(ds))
+    for got, name, dt in ((h, "h", dtype), (s, "state", torch.float32), (dg, "dgate", dtype), (dx, "dcand", dtype), (d0, "dstate", torch.float32)):
+        close(got[pick], ref, name, dt)
+    assert torch.isfinite(h.float()).all() and torch.isfinite(rec).all()
+    if T < 1000:
+        n = 8192 // (-(-D // 128) * -(-T // 16)) // 2       # few enough for one channel a lane
+        for at in range(0, B - n, 3 * n):
+            cut = slice(at, at + n)
+            one = glr_scan(g[cut], x[cut], state[cut], mask=None if mask is None else mask[cut], lengths=None if lengths is None else lengths[cut], cand_act=act)
+            # |h| <= 8 max(1, |state|): both are within 200 half steps of fp32 of it and a rounding of the type
+            assert (one[0].double() - h[cut].double()).abs().max() <= 2 * HALF[dtype] * 8 + 400 * HALF[torch.float32] * 8
+            assert (one[1] - s[cut]).abs().max() <= 400 * HALF[torch.float32] * 8
