@@ -16,25 +16,22 @@ BLOCK = 256      # elements that share a scale of the 8-bit states
 _address = torch.Tensor.data_ptr
 
 
-def _spans(lists):
-    return sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name, i) for name, ts in lists for i, t in enumerate(ts or ()) if t is not None and t.numel())
-
-
 def _apart(lists):
     """Refuses two tensors of the lists that share memory: every one is written by waves of its own.  -> where they lie, in order"""
-    spans = _spans(lists)
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name, i) for name, ts in lists for i, t in enumerate(ts or ()) if t is not None and t.numel())
     for (_, end, a, i), (start, _, b, j) in zip(spans, spans[1:]):
         if start < end:
             raise HierTCNError(f"{a}[{i}] and {b}[{j}] overlap")
     return spans
 
 
-def _clear_of(spans, starts, lists):
-    """Refuses a tensor of the lists that shares memory with one of `spans` (of _apart; starts: their first addresses)."""
-    for start, end, name, i in _spans(lists):
-        k = bisect.bisect_left(starts, end) - 1
-        if k >= 0 and spans[k][1] > start:
-            raise HierTCNError(f"{name}[{i}] and {spans[k][2]}[{spans[k][3]}] overlap")
+def _clear_of(spans, starts, name, places):
+    """Refuses a place (address, bytes) that shares memory with one of `spans` (of _apart; starts: their first addresses)."""
+    for i, (at, size) in enumerate(places):
+        if at and size:
+            k = bisect.bisect_left(starts, at + size) - 1
+            if k >= 0 and spans[k][1] > at:
+                raise HierTCNError(f"{name}[{i}] and {spans[k][2]}[{spans[k][3]}] overlap")
 
 
 class AdamW:
@@ -192,7 +189,7 @@ class AdamW:
                 raise HierTCNError(f"grads[{i}]: a float32, bfloat16 or float16 tensor")
             found.append((None, 0) if g is None else (need(g, f"grads[{i}]", g.dtype, self.device, shape).data_ptr(), _ops.DTYPE[g.dtype]))
         if self._clear.get("grads") != found:         # (sizes are the parameters')
-            _clear_of(self._written, self._starts, (("grads", grads),))
+            _clear_of(self._written, self._starts, "grads", [(ptr, k * (2 if dtype else 4)) for (ptr, dtype), k in zip(found, self._flat_numel)])
             self._clear["grads"] = found
         for d, (ptr, dtype) in zip(self._desc, found):
             d.grad, d.grad_dtype = ptr, dtype
@@ -234,12 +231,14 @@ class AdamW:
                 return out
             return self.m, self.v
         self._follow(states_only=True)
-        if out is None:
+        fresh = out is None
+        if fresh:
             out = tuple([torch.empty(p.numel(), dtype=torch.float32, device=self.device) for p in self.params] for _ in range(2))
         found = [[None if o is None else need(o, "out", torch.float32, self.device, k).data_ptr() for o, k in zip(lst, self._flat)] for lst in out]
-        if self._clear.get("out") != found:
+        if not fresh and self._clear.get("out") != found:
             _apart((("m out", out[0]), ("v out", out[1])))
-            _clear_of(self._written, self._starts, (("m out", out[0]), ("v out", out[1])))
+            for name, ptrs in zip(("m out", "v out"), found):
+                _clear_of(self._written, self._starts, name, [(ptr, 4 * k) for ptr, k in zip(ptrs, self._flat_numel)])
             self._clear["out"] = found
         _ops.call(_ops.lib().hiertcn_adamw_moments, self.device, self._desc, n, *((C.c_void_p * n)(*ptrs) for ptrs in found))
         return out
