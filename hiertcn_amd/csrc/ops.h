@@ -141,5 +141,5 @@ __device__ __forceinline__ float ops_exp(float x) { return __builtin_amdgcn_exp2
 // The same to 3 half steps and |x| / 20: with t = x log2 e as rounded, e^x = 2^t e^(x - t ln 2), whose second factor is 1 + (x - t ln 2) to 2^-33.
 __device__ __forceinline__ float ops_exp_fp32(float x) {
   const float t = x * 1.4426950408889634f, e = __builtin_amdgcn_exp2f(t);
-  return e == 0.f ? e : fmaf(e, fmaf(t, -0.6931471805599453f, x), e);      // (x may be -infinity)
+  return fmaf(e, __builtin_amdgcn_fmed3f(fmaf(t, -0.6931471805599453f, x), -1.f, 1.f), e);      // (t may be -inf, and the inner one infinite or NaN: e is 0 then)
 }
