@@ -10,9 +10,9 @@
 // expectation.  The arithmetic up to the codes is single operations in fp32 without contraction, so that any other implementation of the formula
 // that rounds every operation gets the same codes.
 //
-// 32 bits: bound by memory, 26.7 us for 5.4 M parameters (161 MB in cache, 6 TB/s).  8 bits, 155.5 M parameters with bf16 gradients and copies: 575 us for
+// 32 bits: bound by memory, 26.9 us for 5.4 M parameters (161 MB in cache, 6 TB/s).  8 bits, 155.5 M parameters with bf16 gradients and copies: 579 us for
 // 2.5 GB (4.3 TB/s); by then 545 vector instructions a wave fill nine tenths of the cycles, so the instructions were what was cut (bounds of full blocks, maxima by
-// lane moves, roots and quotients without the library's range handling: 725 -> 545, 706 -> 575 us).  Decoding the moments: 293 us for 1.56 GB, four blocks
+// lane moves, roots and quotients without the library's range handling: 725 -> 545, 706 -> 575 us).  Decoding the moments: 294 us for 1.56 GB, four blocks
 // to a wave (375 us with one).
 #include <math.h>
 

@@ -18,9 +18,9 @@
 // with the same A.  States are not read back from the rounded output: the forward pass leaves the fp32 state before every segment in `record`, 1/16 of
 // a [B][T][D] fp32 array, and a wave replays its segment from there.
 //
-// Bound by memory where the arrays are large and by the latency of a tile (load, fold, replay, store) where they are not: 8.6 / 11.8 us forward / backward at
-// 32 x 200 x 128 fp32, 17.6 / 25.0 at 64 x 500 x 256 bf16, 95 / 157 (4.2 TB/s) at 512 x 500 x 256 bf16, 114 / 198 (3.5 / 3.4 TB/s, half of the cycles in vector
-// instructions) at 2 x 65536 x 512 bf16 chained, 93 / 137 (4.2 / 4.8 TB/s) at 128 x 2000 x 128 fp32; a copy of many GB runs at 4.8.  A single step of 32 x 256: 4.8 us,
+// Bound by memory where the arrays are large and by the latency of a tile (load, fold, replay, store) where they are not: 9.1 / 12.7 us forward / backward at
+// 32 x 200 x 128 fp32, 18.0 / 25.8 at 64 x 500 x 256 bf16, 92 / 159 (4.2 TB/s) at 512 x 500 x 256 bf16, 115 / 199 (3.5 / 3.4 TB/s, half of the cycles in vector
+// instructions) at 2 x 65536 x 512 bf16 chained, 94 / 137 (4.2 / 4.8 TB/s) at 128 x 2000 x 128 fp32; a copy of many GB runs at 4.8.  A single step of 32 x 256: 4.8 us,
 // a launch.  Fetching the next tile before the fold of this one costs registers and waves: 114 -> 155 chained, nothing gained elsewhere.
 //
 // A reset has to cut a state that is NaN or infinite (0 * NaN = NaN), and nothing else may: A is exactly 0 only where a reset lies in the run, and a map with A = 0
@@ -479,7 +479,11 @@ struct Plan { int vec, nw; bool chain; int64_t ncb, ntile; };
 //   one workgroup through a sequence where there are 256 of them: 64 x 500 x 256 19 / 28 against 25 / 35 chained; chained where there are fewer:
 //   2 x 65536 x 512 116 / 190 against 1670 / 2210, 8 x 500 x 256 12 / 14 against 16 / 23
 //   waves of a workgroup: as few as make 4096 in all (4096 x 30 x 256 one: 49 / 76, two 65 / 130 before; 512 x 500 x 256 four: 95 / 153, eight 97 / 160); chained
-//   eight (2 x 65536 x 512 132 / 189 against 160 / 215 with sixteen), but sixteen where those are one generation of workgroups (17 x 1001 x 333 24 against 27)
+//   eight (2 x 65536 x 512 132 / 189 against 160 / 215 with sixteen), but sixteen where 256 to 512 workgroups of sixteen make it all: the chain is half as long.  Sixteen
+//   against eight, with k_chain_init: 17 x 1001 x 333 fp16 24.8 / 32.4 against 27.6 / 32.2, 8 x 1001 x 512 bf16 17.5 / 20.9 against 19.9 / 23.0, 4 x 4000 x 256 bf16
+//   18.3 / 22.1 against 20.7 / 24.1, 2 x 20000 x 128 fp32 27.7 / 34.4 against 31.2 / 33.6, 40 x 700 x 200 fp32 26.3 / 36.6 against 29.5 / 34.5, 1 x 130000 x 64 bf16
+//   46 / 49 against 82 / 80; the one loss of nine shapes 12 x 1500 x 256 fp32, 25.5 / 32.3 against 24.6 / 28.2.  (A compute unit holds one workgroup of sixteen waves of
+//   75 to 107 registers, so up to 256 of them are resident and the others follow.)
 Plan plan_of(int64_t B, int64_t T, int64_t D, bool wide, bool backward) {
   Plan q{};
   const int64_t nseg = (T + SEG - 1) / SEG;

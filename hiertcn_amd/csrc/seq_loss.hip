@@ -9,8 +9,8 @@
 // Masked rows are not read: their gradient rows are written as zeros.  All sums run in a fixed order.
 //
 // Bound by memory: the answered rows are read twice (c needs a whole row, a pair's needs two sequences), all gradient rows written once.  64 x 30 x 300000 bf16,
-// half of the rows answered: k_part 91 us for 0.58 GB (some of it in the last cache), k_policy 7, k_dlogits 279 for 1.73 GB (6.2 TB/s); 8 pairs x 30 x 300000
-// fp32: 33, 10, 113.  At 16 pairs x 20 x 20778 bf16 and below it is three launches of 4 to 8 us.  (A single pass that keeps the rows in registers while their
+// half of the rows answered: k_part 91 us for 0.58 GB (some of it in the last cache), k_policy 7, k_dlogits 280 for 1.73 GB (6.2 TB/s); 8 pairs x 30 x 300000
+// fp32: 35, 9.5, 114.  At 16 pairs x 20 x 20778 bf16 and below it is three launches of 4 to 8 us.  (A single pass that keeps the rows in registers while their
 // workgroups wait for one another is no faster: 461 us against 463 in two passes at the first of these, before the stores were taken past the caches.)
 #include <math.h>
 

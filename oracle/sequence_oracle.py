@@ -1,8 +1,9 @@
 """64-bit restatement of the sequence operators (include/hiertcn_ops.h) in NumPy, one step after the other -- test infrastructure only.
 
 Where a function also returns a bound, it is the error that 32-bit arithmetic may leave there, carried along with the value itself:
-EPS = 2^-24 is half a step of fp32, and a sigmoid or tanh of |x| <= 8 built from exp2, a reciprocal and a few products is within
-(|x| + 8) EPS of itself (|x| EPS from rounding x log2 e, one step each for exp2 and the reciprocal, half a step for every product and sum)."""
+EPS = 2^-24 is half a step of fp32, and a sigmoid or tanh built from exp2, a reciprocal and a few products is within 16 EPS of itself: one step each for
+exp2 and the reciprocal, half a step for every product and sum, and the rounding of x log2 e, which is |x| EPS where nothing is done about it (16-bit operands:
+|x| <= 8 here) and |x| / 20 EPS where it is taken back (fp32 operands: up to |x| = 80)."""
 from __future__ import annotations
 
 import numpy as np
@@ -79,7 +80,8 @@ def answered(ids, V):
 
 def rows(logits, ids):
     """-> dict: logp [n, T] with its bound, live (answered, and not all -inf), p [n, T, V] with its RELATIVE bound.  A sum of positive terms of at most
-    32 elements a thread, joined over lanes, waves and at most 64 parts, is within 120 half steps of itself; an exponential within 2 (|x| + 4)."""
+    32 elements a thread, joined over lanes, waves and at most 64 parts, is within 120 half steps of itself (a thread takes up to 128 where rows are many: 96 more, which
+    the callers add); an exponential within 2 (|x| + 4)."""
     z = np.asarray(logits, np.float64)
     n, T, V = z.shape
     ok = answered(ids, V)
