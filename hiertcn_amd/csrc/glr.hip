@@ -18,7 +18,7 @@
 // with the same A.  States are not read back from the rounded output: the forward pass leaves the fp32 state before every segment in `record`, 1/16 of
 // a [B][T][D] fp32 array, and a wave replays its segment from there.
 //
-// Bound by memory where the arrays are large and by the latency of a tile (load, fold, replay, store) where they are not: 9.1 / 12.7 us forward / backward at
+// Bound by memory where the arrays are large and by the latency of a tile (load, fold, replay, store) where they are not: 8.9 / 12.5 us forward / backward at
 // 32 x 200 x 128 fp32, 18.0 / 25.8 at 64 x 500 x 256 bf16, 92 / 159 (4.2 TB/s) at 512 x 500 x 256 bf16, 115 / 199 (3.5 / 3.4 TB/s, half of the cycles in vector
 // instructions) at 2 x 65536 x 512 bf16 chained, 94 / 137 (4.2 / 4.8 TB/s) at 128 x 2000 x 128 fp32; a copy of many GB runs at 4.8.  A single step of 32 x 256: 4.8 us,
 // a launch.  Fetching the next tile before the fold of this one costs registers and waves: 114 -> 155 chained, nothing gained elsewhere.
@@ -58,13 +58,11 @@ __device__ __forceinline__ float map_a(float A1, float A2) { return !CUT ? fmaxf
 template <bool CUT>
 __device__ __forceinline__ float map_s(float A2, float S1, float S2) { return CUT && A2 == 0.f ? S2 : fmaf(A2, S1, S2); }
 
-// exp of what is at most 0.  Behind 16-bit operands |x| half steps of fp32 are 2^-13 of the operand's own (4096 x 30 x 256 bf16 43 / 71 us, 49 / 77 with the better one)
-template <int DT>
-__device__ __forceinline__ float exp_of(float x) { return DT == HIERTCN_FP32 ? ops_exp_fp32(x) : ops_exp(x); }
+// (The exponential of 16-bit operands is |x| half steps of fp32 off, 2^-13 or less of the operand's own: 4096 x 30 x 256 bf16 43 / 71 us, 49 / 77 with the better one.)
 // u = sigmoid(g) and w = 1 - u = sigmoid(-g), each to 8 half steps and what the exponential adds (1 - u formed from u would lose the small ones)
 template <int DT>
 __device__ __forceinline__ void gate_of(float g, float& u, float& w) {
-  const float e = exp_of<DT>(-fabsf(g));
+  const float e = ops_exp_of<DT>(-fabsf(g));
   const float r = __builtin_amdgcn_rcpf(1.f + e), er = e * r;
   u = g >= 0.f ? r : er;
   w = g >= 0.f ? er : r;
@@ -74,7 +72,7 @@ __device__ __forceinline__ void gate_of(float g, float& u, float& w) {
 template <int DT>
 __device__ __forceinline__ float tanh_of(float x, float& slope) {
   const float a = fabsf(x), x2 = x * x;
-  const float e = exp_of<DT>(-2.f * a);
+  const float e = ops_exp_of<DT>(-2.f * a);
   const float r = __builtin_amdgcn_rcpf(1.f + e);
   const float big = copysignf((1.f - e) * r, x);
   slope = 4.f * e * r * r;

@@ -143,3 +143,6 @@ __device__ __forceinline__ float ops_exp_fp32(float x) {
   const float t = x * 1.4426950408889634f, e = __builtin_amdgcn_exp2f(t);
   return fmaf(e, __builtin_amdgcn_fmed3f(fmaf(t, -0.6931471805599453f, x), -1.f, 1.f), e);      // (t may be -inf, and the inner one infinite or NaN: e is 0 then)
 }
+// the one of the two that operands of type DT are worth
+template <int DT>
+__device__ __forceinline__ float ops_exp_of(float x) { return DT == HIERTCN_FP32 ? ops_exp_fp32(x) : ops_exp(x); }

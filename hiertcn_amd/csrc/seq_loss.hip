@@ -10,7 +10,7 @@
 //
 // Bound by memory: the answered rows are read twice (c needs a whole row, a pair's needs two sequences), all gradient rows written once.  64 x 30 x 300000 bf16,
 // half of the rows answered: k_part 91 us for 0.58 GB (some of it in the last cache), k_policy 7, k_dlogits 280 for 1.73 GB (6.2 TB/s); 8 pairs x 30 x 300000
-// fp32: 35, 9.5, 114.  At 16 pairs x 20 x 20778 bf16 and below it is three launches of 4 to 8 us.  (A single pass that keeps the rows in registers while their
+// fp32: 34, 9.8, 114.  At 16 pairs x 20 x 20778 bf16 and below it is three launches of 4 to 8 us.  (A single pass that keeps the rows in registers while their
 // workgroups wait for one another is no faster: 461 us against 463 in two passes at the first of these, before the stores were taken past the caches.)
 #include <math.h>
 
@@ -46,10 +46,6 @@ __device__ __forceinline__ bool answered(const hiertcn_rows_t& a, int64_t r, int
   y = a.ids[r];
   return y > 0 && y < a.V;
 }
-
-// exp of what is at most 0.  fp32 logits: to 3 half steps wherever it lies; 16-bit ones: |x| half steps of fp32 more, behind a rounding of 2^13 or more of them
-template <int DT>
-__device__ __forceinline__ float exp_of(float x) { return DT == HIERTCN_FP32 ? ops_exp_fp32(x) : ops_exp(x); }
 
 // (m, s) of two runs as one.  m = -inf: nothing in it (s is 0, or NaN and stays NaN).
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
@@ -119,12 +115,12 @@ __device__ __forceinline__ void fold(const typename OpsRaw<DT, VEC>::type (&x)[U
     }
   }
   const float ref = ref_of(top);
-  s *= exp_of<DT>(m - ref);
+  s *= ops_exp_of<DT>(m - ref);
   m = top;
 #pragma unroll
   for (int u = 0; u < U; u++)
 #pragma unroll
-    for (int i = 0; i < VEC; i++) s += exp_of<DT>(z[u][i] - ref);
+    for (int i = 0; i < VEC; i++) s += ops_exp_of<DT>(z[u][i] - ref);
 }
 
 // answers per sequence, and this workgroup's share of their totals: a thread a sequence where sequences are short, else a wave
@@ -400,7 +396,7 @@ __device__ __forceinline__ void gradient_of(const typename OpsRaw<DT, VEC>::type
   float z[VEC];
   ops_cvt<DT, VEC>(x, z);
 #pragma unroll
-  for (int i = 0; i < VEC; i++) z[i] = g * exp_of<DT>(z[i] - ref);
+  for (int i = 0; i < VEC; i++) z[i] = g * ops_exp_of<DT>(z[i] - ref);
   if (y >= at && y - at < VEC)
 #pragma unroll
     for (int i = 0; i < VEC; i++) z[i] += i == y - at ? c : 0.f;
@@ -455,7 +451,7 @@ __global__ __launch_bounds__(NT) void k_dlogits(RowsP p, Sums q) {
   if (e >= 0) {
     float z[1];
     ops_ld<DT, 1>(row, e, z);
-    z[0] = g * exp_of<DT>(z[0] - ref);
+    z[0] = g * ops_exp_of<DT>(z[0] - ref);
     if (e == y) z[0] += c;
     ops_st<DT, 1>(out, e, z);
   }
