@@ -128,7 +128,7 @@ class AdamW:
         self._watched = theirs + [t for t in (*self.params, *self.copies, *(self.grads or ())) if t is not None]
         self._watched_states = len(theirs)
         self._at = [*map(_address, self._watched)]
-        self._held = [t.detach() for t in (*self._watched, *states)]
+        self._held = [t.untyped_storage() for t in (self._watched if self._callers else self._watched + states)]
 
     def _follow(self, states_only: bool = False):
         """Takes tensors that have other memory than at the last look anew."""
